@@ -1158,3 +1158,10 @@ def moe_combine(y: torch.Tensor, inv_idx: torch.Tensor, w: torch.Tensor, T: int)
 
 def softmax_scale(head_dim: int) -> float:
     return 1.0 / math.sqrt(head_dim)
+
+
+# ---------------------------------------------------------------- the 8-bit KV cache (kv8.py), controls of logits (logits.py)
+
+from .kv8 import (KV8, flash_prefill_kv8, kv8_block_bytes, kv8_cache, paged_decode_fused_kv8, paged_decode_kv8,  # noqa: E402
+                  rope_and_cache_kv8)
+from .logits import LogitControls, allowed_mask, cache_tokens, control_logits, logit_controls  # noqa: E402

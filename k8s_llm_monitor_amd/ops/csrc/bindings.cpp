@@ -981,8 +981,11 @@ void car_error_async(int64_t state, torch::Tensor host) {
 
 void car_destroy(int64_t state) { k8sllm_car_destroy((void*)(intptr_t)state); }
 
+void bind_serving(pybind11::module_& m);  // bindings_serving.cpp
+
 PYBIND11_MODULE(_k8sllm_ops, m) {
   m.doc() = "gfx950 HIP kernels for k8s-llm-monitor-amd";
+  bind_serving(m);
   m.def("rms_norm", &rms_norm);
   m.def("fused_add_rms_norm", &fused_add_rms_norm);
   m.def("layer_norm", &layer_norm);

@@ -103,10 +103,11 @@ __device__ int sample_row_filtered(const T* __restrict__ x, int V, float temp, i
   for (int i = tid; i < V; i += kST) {
     const float v = ld<T>(x, i) * itemp;
     mx = fmaxf(mx, v);
-    mn = fminf(mn, v);
+    mn = fminf(mn, v > -INFINITY ? v : INFINITY);  // masked tokens set no end to the bisections
   }
   mx = block_max<kST>(mx, sv);
   mn = -block_max<kST>(-mn, sv);
+  if (mn > mx) k = 0, p = 1.f;  // every token masked: nothing to filter
   float thr = -INFINITY;
   if (k > 0 && k < V) {
     float lo = mn, hi = mx;  // invariant: count(x >= lo) >= k

@@ -1,0 +1,239 @@
+"""Controls of logits against a plain 64-bit form of their definition.
+
+Tolerance: four roundings of 32-bit arithmetic (quotient or product, frequency * count, two sums or the bias), each half a step (2^-24) of a value that is at
+most the sum of the terms' magnitudes; outputs in bf16 are then off by half a bf16 step of the result more.
+"""
+import math
+
+import pytest
+import torch
+
+from k8s_llm_monitor_amd import ops
+
+DEVICES = ["cpu", pytest.param("cuda", marks=pytest.mark.gpu)]
+
+
+def plain(logits, ctl, rows, tokens, table, lens):
+    """(controlled logits, sum of the terms' magnitudes) in 64 bits; ctl[slot] = (prompt, repetition, presence, frequency, bias, allowed)."""
+    y = logits.double().clone()
+    mag = y.abs()
+    B, V = y.shape
+    for b in range(B):
+        if not 0 <= rows[b] < len(ctl):
+            continue
+        prompt, rep, pres, freq, bias, allowed = ctl[rows[b]]
+        seen, count = set(), {}
+        for t in range(max(0, min(lens[b], len(table[b]) * 16))):
+            page = table[b][t // 16]
+            if not 0 <= page < tokens.shape[0]:
+                continue
+            v = int(tokens[page, t % 16])
+            if 0 <= v < V:
+                seen.add(v)
+                if t >= prompt:
+                    count[v] = count.get(v, 0) + 1
+        for v in seen:
+            x = float(y[b, v])
+            y[b, v] = x / rep if x > 0 else x * rep
+            mag[b, v] = abs(float(y[b, v]))
+        for v, n in count.items():
+            y[b, v] -= freq * n + pres
+            mag[b, v] += abs(freq) * n + abs(pres)
+        for v, x in bias.items():
+            if v < V:
+                y[b, v] += x
+                mag[b, v] += abs(x) if math.isfinite(x) else 0
+        if allowed is not None:
+            keep = torch.zeros(V, dtype=torch.bool)
+            keep[[v for v in allowed if v < V]] = True
+            y[b, ~keep] = -math.inf
+    return y, mag
+
+
+def check(got, want, mag):
+    out16 = got.dtype == torch.bfloat16
+    got = got.cpu().double()
+    assert torch.equal(got.isnan(), want.isnan())
+    inf = want.isinf()
+    assert torch.equal(got[inf], want[inf])
+    ok = want.isfinite()
+    bound = 5 * 2.0 ** -24 * mag + (torch.finfo(torch.bfloat16).eps / 2 * (want.abs() + 2.0 ** -20 * mag) if out16 else 0) + 2.0 ** -126
+    assert bool(((got - want).abs() <= bound)[ok].all())
+
+
+def controls(dev, V, ctl, max_bias=8):
+    c = ops.logit_controls(len(ctl), V, max_bias, device=dev)
+    for i, (prompt, rep, pres, freq, bias, allowed) in enumerate(ctl):
+        c.set(i, prompt, rep, pres, freq, bias, allowed)
+    return c
+
+
+f32 = lambda x: float(torch.tensor(x, dtype=torch.float32))  # noqa: E731
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+@pytest.mark.parametrize("V", [1, 7, 255, 2048, 2049, 5003, 33000])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_rows_of_every_kind(dev, V, dtype):
+    gen = torch.Generator().manual_seed(V)
+    lens = [0, 1, 40, 300, 64, 300, 1000]
+    B, pages = len(lens), 30
+    ctl = [(3, f32(1.3), 0.5, 0.25, {}, None),
+           (0, f32(0.8), -0.5, f32(0.1), {0: 2.5, V - 1: -100.0, V // 2: math.inf, V + 7: 1.0}, None),
+           (1000, 1.0, 0.0, 0.0, {V // 3: f32(0.3)}, sorted(set(torch.randint(0, V, (5,), generator=gen).tolist()))),
+           (20, f32(2.2), f32(0.7), f32(0.3), {v: float(v % 5) for v in range(min(8, V))}, []),
+           (250, f32(1.1), 1.0, 1.0, {}, range(0, V, 2))]
+    rows = [0, 1, 2, -1, 3, 4, 5]  # 5: outside the slots
+    if V == 1:
+        ctl[1] = (0, f32(0.8), -0.5, f32(0.1), {0: 2.5}, None)
+    tokens = (V * torch.rand(pages, 16, generator=gen) ** 4).int()
+    tokens[3] = torch.tensor([-1, V, 1 << 30, -(1 << 31)] * 4, dtype=torch.int32)  # ids outside the vocabulary
+    table = torch.randint(0, pages, (B, 20), generator=gen).int()
+    table[5, 2], table[5, 3] = -1, pages  # pages outside the cache
+    logits = (4 * torch.randn(B, V, generator=gen)).to(dtype)
+    logits[2, V // 2] = math.nan  # masked or not
+    logits[4] = -math.inf
+    want, mag = plain(logits, ctl, rows, tokens, table.tolist(), lens)
+    c = controls(dev, V, ctl)
+    args = (c, torch.tensor(rows, dtype=torch.int32, device=dev), tokens.to(dev), table.to(dev), torch.tensor(lens, dtype=torch.int32, device=dev))
+    x = logits.to(dev)
+    got = ops.control_logits(x, *args)
+    check(got, want, mag)
+    assert torch.equal(x.cpu().nan_to_num(), logits.nan_to_num())
+    check(ops.control_logits(x, *args, out=torch.empty(B, V, device=dev)), want, mag)
+    # rows that do not start at 16 bytes, and rows of a wider buffer, which keeps the rest
+    wide = torch.full((B, V + 13), 3.0, dtype=dtype, device=dev)
+    wide[:, 5:5 + V] = x
+    view = wide[:, 5:5 + V]
+    assert ops.control_logits(view, *args, out=view) is view
+    check(view, want, mag)
+    assert bool((wide[:, :5] == 3).all()) and bool((wide[:, 5 + V:] == 3).all())
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+def test_a_token_many_times_and_a_long_history(dev):
+    V, n = 4099, 9000
+    tokens = torch.full((n // 16 + 1, 16), 4000, dtype=torch.int32)
+    tokens[7] = 11
+    table = torch.arange(n // 16 + 1, dtype=torch.int32)[None]
+    logits = torch.linspace(-3, 3, V)[None].contiguous()
+    ctl = [(100, 1.5, 0.25, 2.0 ** -10, {4000: 1.0}, None)]
+    want, mag = plain(logits, ctl, [0], tokens, table.tolist(), [n])
+    got = ops.control_logits(logits.to(dev), controls(dev, V, ctl), torch.zeros(1, dtype=torch.int32, device=dev), tokens.to(dev), table.to(dev),
+                             torch.tensor([n], dtype=torch.int32, device=dev))
+    check(got, want, mag)
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+def test_of_several_entries_with_one_token_the_first_counts(dev):
+    c = ops.logit_controls(1, 300, 4, device=dev)
+    c.bias_ids[0] = torch.tensor([9, 5, 9, 5], dtype=torch.int32)
+    c.bias_vals[0] = torch.tensor([1.0, 2.0, 4.0, 8.0])
+    z = torch.zeros(1, 1, dtype=torch.int32, device=dev)
+    got = ops.control_logits(torch.zeros(1, 300, device=dev), c, z[0], torch.zeros(1, 16, dtype=torch.int32, device=dev), z, z[0])
+    want = torch.zeros(300)
+    want[9], want[5] = 1.0, 2.0
+    assert torch.equal(got[0].cpu(), want)
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+def test_the_token_cache(dev):
+    cache = torch.full((4, 16), -9, dtype=torch.int32, device=dev)
+    i32 = lambda *v: torch.tensor(v, dtype=torch.int32, device=dev)  # noqa: E731
+    ops.cache_tokens(cache, i32(5, 6, 7, 8, 9), i32(17, -1, 63, 64, 0))
+    want = torch.full((4, 16), -9, dtype=torch.int32)
+    want[1, 1], want[3, 15], want[0, 0] = 5, 7, 9
+    assert torch.equal(cache.cpu(), want)
+    # decode rows whose input is what the step before sampled
+    ops.cache_tokens(cache, i32(1, 2, 3), i32(2, 3, 4), src=i32(-1, 1, 0), prev=i32(70, 71))
+    want[0, 2], want[0, 3], want[0, 4] = 1, 71, 70
+    assert torch.equal(cache.cpu(), want)
+    ops.cache_tokens(cache, i32(1, 2, 3)[:0], i32(2, 3, 4)[:0])
+    assert torch.equal(cache.cpu(), want)
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+@pytest.mark.parametrize("top_k,top_p", [(0, 1.0), (3, 1.0), (0, 0.9), (50, 0.5)])
+def test_sampling_behind_a_mask(dev, top_k, top_p):
+    """The sampler takes allowed tokens only - also with top-k and top-p, whose thresholds a row's infinities must not hide - and the lowest of
+    a row that allows none."""
+    V, B = 1500, 6
+    gen = torch.Generator().manual_seed(top_k)
+    allowed = [sorted(set(torch.randint(0, V, (n,), generator=gen).tolist())) for n in (1, 2, 40, 700, 0)]
+    c = controls(dev, V, [(0, 1.0, 0.0, 0.0, {}, a) for a in allowed])
+    x = (2 * torch.randn(B, V, generator=gen)).to(dev)
+    z = torch.zeros(B, 1, dtype=torch.int32, device=dev)
+    y = ops.control_logits(x, c, torch.tensor([0, 1, 2, 3, 4, -1], dtype=torch.int32, device=dev), torch.zeros(1, 16, dtype=torch.int32, device=dev), z, z[:, 0].contiguous())
+    assert ops.sample(y).tolist()[:5] == [max(a, key=lambda v: float(x[b, v])) if a else 0 for b, a in enumerate(allowed)]
+    full = lambda v, t: torch.full((B,), v, dtype=t, device=dev)  # noqa: E731
+    temps = full(1.5, torch.float32)
+    if dev == "cpu":
+        y = y[:4]  # (a row of nothing has no distribution to draw from there)
+    best = [torch.topk(y[b].float(), min(top_k, len(allowed[b]))).indices.tolist() if top_k else allowed[b] for b in range(4)]
+    rng = torch.tensor([1, 0], dtype=torch.int64, device=dev)
+    for _ in range(30):
+        t = ops.sample(y, temps, full(top_k, torch.int32), full(top_p, torch.float32), rng, advance=True).tolist()
+        for b in range(4):
+            assert t[b] in best[b]
+        assert dev == "cpu" or t[4] == 0
+
+
+def test_refused_controls():
+    c = ops.logit_controls(2, 100, 3)
+    for bad in (dict(repetition=0.0), dict(repetition=math.nan), dict(presence=math.inf), dict(frequency=math.nan), dict(bias={-1: 1.0}),
+                dict(bias={3: math.nan}), dict(bias={i: 1.0 for i in range(4)}), dict(allowed=[128]), dict(allowed=[-1])):
+        with pytest.raises(ValueError):
+            c.set(0, 5, **bad)
+    with pytest.raises(ValueError):
+        c.set(2, 5)
+    with pytest.raises(ValueError):
+        ops.logit_controls(1, 10, 5000)
+    assert c.info.tolist() == [[0, 0], [0, 0]]
+
+
+@pytest.mark.gpu
+def test_refused_calls():
+    dev, B, V = "cuda", 2, 300
+    z = lambda *s: torch.zeros(*s, dtype=torch.int32, device=dev)  # noqa: E731
+    c = ops.logit_controls(2, V, 3, device=dev)
+    base = dict(logits=torch.zeros(B, V, device=dev), controls=c, rows=z(B), token_cache=z(4, 16), block_tables=z(B, 2), seq_lens=z(B))
+    ops.control_logits(**base)
+    for bad in (dict(logits=torch.zeros(B, V, dtype=torch.float16, device=dev)), dict(logits=torch.zeros(V, B, device=dev).t()), dict(rows=z(1)),
+                dict(rows=z(B).long()), dict(token_cache=z(4, 8)), dict(block_tables=z(1, 2)), dict(seq_lens=z(1)), dict(out=torch.zeros(B, V + 1, device=dev)),
+                dict(out=torch.zeros(B, V, dtype=torch.bfloat16, device=dev)), dict(controls=c._replace(masks=z(2, 9))),
+                dict(controls=c._replace(bias_vals=c.bias_vals[:, :2])), dict(controls=c._replace(params=c.params.cpu())),
+                dict(block_tables=z(B, 1 << 16))):
+        with pytest.raises(RuntimeError):
+            ops.control_logits(**{**base, **bad})
+    with pytest.raises(RuntimeError):
+        ops.cache_tokens(z(4, 16), z(3), z(2))
+    with pytest.raises(RuntimeError):
+        ops.cache_tokens(z(4, 16), z(3), z(3), src=z(3))
+    torch.cuda.synchronize()
+
+
+@pytest.mark.gpu
+def test_replays_in_a_graph():
+    dev, B, V = "cuda", 3, 5003
+    gen = torch.Generator().manual_seed(5)
+    ctl = [(4, f32(1.3), 0.5, 0.25, {7: 1.0}, range(0, V, 3))]
+    c = controls(dev, V, ctl)
+    tokens, table = torch.zeros(6, 16, dtype=torch.int32, device=dev), torch.arange(6, dtype=torch.int32, device=dev).view(3, 2)
+    rows, lens = torch.tensor([0, -1, 0], dtype=torch.int32, device=dev), torch.tensor([20, 3, 32], dtype=torch.int32, device=dev)
+    x, out = torch.zeros(B, V, device=dev), torch.zeros(B, V, device=dev)
+    ids, slots = torch.zeros(3, dtype=torch.int32, device=dev), torch.tensor([19, 34, 95], dtype=torch.int32, device=dev)
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        ops.cache_tokens(tokens, ids, slots)
+        ops.control_logits(x, c, rows, tokens, table, lens, out=out)
+    for _ in range(4):
+        xs, old = torch.randn(B, V, generator=gen), torch.randint(0, V, (6, 16), generator=gen).int()
+        new = torch.randint(0, V, (3,), generator=gen).int()
+        x.copy_(xs)
+        tokens.copy_(old)
+        ids.copy_(new)
+        g.replay()
+        torch.cuda.synchronize()
+        old.view(-1)[[19, 34, 95]] = new
+        check(out, *plain(xs, ctl, rows.tolist(), old, table.tolist(), lens.tolist()))
