@@ -123,38 +123,53 @@ __global__ __launch_bounds__(256, 2) void kv8_decode_kernel(const Kv8Decode a) {
   const int* bt = a.table + (long)b * a.table_stride;
   const int last_page = (len - 1) >> 4;
 
-  // page numbers of the wave's step: K's (page col >> 2) and V's (page kg).  Ones past the end are the last page's, and those outside the
-  // cache are held to its ends.
+  // page numbers of the wave's step: K's (page col >> 2) and V's (page kg).  Ones past the end are the last page's; those outside the
+  // cache are held to its ends where they are used (here that would be waiting for them).
   auto pages_of = [&](int c, int* pk, int* pv) {
     const int p0 = (c * kChunk + wave * kStep) >> 4;
-    *pk = min(max(bt[min(p0 + (col >> 2), last_page)], 0), a.pages - 1);
-    *pv = min(max(bt[min(p0 + kg, last_page)], 0), a.pages - 1);
+    *pk = bt[min(p0 + (col >> 2), last_page)];
+    *pv = bt[min(p0 + kg, last_page)];
   };
-  auto issue = [&](Kv8Tiles<D>& t, int pk, int pv) {
-    const long kt = (long)pk * a.Hkv + kvh, vt = (long)pv * a.Hkv + kvh;
-    const uint8_t* kp = a.k + kt * (kPage * D) + (kg * kPage + (col & 3)) * KD;
+  auto issue = [&](Kv8Tiles<D>& t, int c, int pk, int pv) {
+    const bool real = c < c1;  // uniform
+    const long kt = (long)min(max(pk, 0), a.pages - 1) * a.Hkv + kvh, vt = (long)min(max(pv, 0), a.pages - 1) * a.Hkv + kvh;
+    t.ks = a.scales[kt * 2];
+    t.vs = a.scales[vt * 2 + 1];
+    const uint8_t* kp = a.k + kt * (kPage * D) + (real ? (kg * kPage + (col & 3)) * KD : 0);
 #pragma unroll
     for (int i = 0; i < 4; ++i)
 #pragma unroll
       for (int w = 0; w < KW; ++w) t.k[i][w] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(kp + 4 * i * KD + 16 * w));
-    const uint8_t* vp = a.v + vt * (kPage * D) + col * kPage;
+    const uint8_t* vp = a.v + vt * (kPage * D) + (real ? col * kPage : 0);
 #pragma unroll
     for (int d = 0; d < DT; ++d) t.v[d] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(vp + d * 16 * kPage));
-    t.ks = a.scales[kt * 2];
-    t.vs = a.scales[vt * 2 + 1];
   };
-  Kv8Tiles<D> t0, t1;
-  int pk, pv;
-  pages_of(c0, &pk, &pv);
-  issue(t0, pk, pv);
-  if (c0 + 1 < c1) {
-    pages_of(c0 + 1, &pk, &pv);
-    issue(t1, pk, pv);
-  }
-  pages_of(min(c0 + 2, c1 - 1), &pk, &pv);
-
   bf16x8 qf[KS];
   const int hc = min(col, G - 1);
+  if constexpr (!FUSED) {
+    const bf16_t* qp = a.q + (long)b * a.q_stride + (long)(kvh * G + hc) * D + KD * kg;
+#pragma unroll
+    for (int s = 0; s < KS; ++s) qf[s] = *reinterpret_cast<const bf16x8*>(qp + 8 * s);
+  }
+  // Loads return in order and the compiler counts them, so every path through the loop issues the same ones: behind the last step all lanes
+  // read one place of the last page.  A buffer's page numbers are asked for behind its data, a turn before they are used.
+  Kv8Tiles<D> t0, t1;
+  int k0, v0, k1, v1, kn, vn;
+  pages_of(c0, &k0, &v0);
+  pages_of(c0 + 1, &k1, &v1);
+  pages_of(c0 + 2, &kn, &vn);
+  issue(t0, c0, k0, v0);
+  k0 = kn, v0 = vn;
+  pages_of(c0 + 3, &kn, &vn);
+  __builtin_amdgcn_sched_barrier(0);  // t0's loads stay ahead of t1's, here as in the loop
+  issue(t1, c0 + 1, k1, v1);
+  k1 = kn, v1 = vn;
+  __builtin_amdgcn_sched_barrier(0);
+  auto refill = [&](Kv8Tiles<D>& t, int c, int& pk, int& pv) {
+    issue(t, c, pk, pv);
+    pages_of(c + 2, &pk, &pv);
+  };
+
   float k_old = 0.f, v_old = 0.f, k_new = 0.f, v_new = 0.f;
   int slot = -1;
   if constexpr (FUSED) {
@@ -214,10 +229,9 @@ __global__ __launch_bounds__(256, 2) void kv8_decode_kernel(const Kv8Decode a) {
         *reinterpret_cast<bf16x4*>(&s_kv[lane >> 5][d]) = bf16x4{lo[0], lo[1], hi[0], hi[1]};
       }
     }
-  } else {
-    const bf16_t* qp = a.q + (long)b * a.q_stride + (long)(kvh * G + hc) * D + KD * kg;
+  } else {  // q has arrived before the loop, whose first wait for it would else stand for every load in flight
 #pragma unroll
-    for (int s = 0; s < KS; ++s) qf[s] = *reinterpret_cast<const bf16x8*>(qp + 8 * s);
+    for (int s = 0; s < KS; ++s) asm volatile("" ::"v"(qf[s]));
   }
 
   float m = -1e30f, l = 0.f;  // of head `col`
@@ -304,22 +318,19 @@ __global__ __launch_bounds__(256, 2) void kv8_decode_kernel(const Kv8Decode a) {
       t.vs = v_new;
     }
   };
-  for (int c = c0; c < c1; c += 2) {
-    if (FUSED && grew && c + 1 == c1) renew(t0, c);
+  int c = c0;
+  for (; c + 1 < c1; c += 2) {  // (no way out in the middle: it would join the loop's head with fewer loads behind it)
     compute(t0, c);
-    if (c + 2 < c1) {
-      issue(t0, pk, pv);
-      pages_of(min(c + 3, c1 - 1), &pk, &pv);
-    }
+    refill(t0, c + 2, k0, v0);
     __builtin_amdgcn_sched_barrier(0);
-    if (c + 1 >= c1) break;
     if (FUSED && grew && c + 2 == c1) renew(t1, c + 1);
     compute(t1, c + 1);
-    if (c + 3 < c1) {
-      issue(t1, pk, pv);
-      pages_of(min(c + 4, c1 - 1), &pk, &pv);
-    }
+    refill(t1, c + 3, k1, v1);
     __builtin_amdgcn_sched_barrier(0);
+  }
+  if (c < c1) {
+    if (FUSED && grew) renew(t0, c);
+    compute(t0, c);
   }
 
   if constexpr (FUSED) {
