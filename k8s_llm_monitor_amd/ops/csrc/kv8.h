@@ -43,6 +43,24 @@ __device__ __forceinline__ uint32_t kv8_codes(float a, float b, float c, float d
   return __builtin_amdgcn_cvt_pk_fp8_f32(c, d, __builtin_amdgcn_cvt_pk_fp8_f32(a, b, 0, false), true);
 }
 
+// Two packed pairs of bf16 numbers over s, as above: the conversion takes bf16 as it lies and s with it.  Infinities and NaN are NaN codes.
+typedef short s16x2 __attribute__((ext_vector_type(2)));
+__device__ __forceinline__ uint32_t kv8_codes_bf16(uint32_t a, uint32_t b, float s) {
+  s16x2 r = __builtin_amdgcn_cvt_scalef32_pk_fp8_bf16(s16x2{0, 0}, __builtin_bit_cast(bf16x2, a), s, false);
+  r = __builtin_amdgcn_cvt_scalef32_pk_fp8_bf16(r, __builtin_bit_cast(bf16x2, b), s, true);
+  return __builtin_bit_cast(uint32_t, r);
+}
+
+// Larger magnitudes of packed bf16 pairs, as 16-bit patterns; 0x7f80 and more: not finite
+typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
+__device__ __forceinline__ uint32_t kv8_max_bits(uint32_t m, uint32_t w) {
+  return __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(u16x2, m), __builtin_bit_cast(u16x2, w & 0x7fff7fffu)));
+}
+__device__ __forceinline__ uint32_t kv8_finite_bits(uint32_t w) {  // numbers that are not finite as zeros
+  const uint32_t lo = (w & 0x7f80u) == 0x7f80u ? 0u : w & 0xffffu, hi = (w & 0x7f800000u) == 0x7f800000u ? 0u : w & 0xffff0000u;
+  return lo | hi;
+}
+
 // Codes under a scale that grew: ratio = old / new
 __device__ __forceinline__ uint32_t kv8_again(uint32_t w, float ratio) {
   const f32x2 a = __builtin_amdgcn_cvt_pk_f32_fp8(w, false), b = __builtin_amdgcn_cvt_pk_f32_fp8(w, true);

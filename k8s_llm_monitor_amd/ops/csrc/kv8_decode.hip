@@ -108,6 +108,9 @@ __global__ __launch_bounds__(256, 2) void kv8_decode_kernel(const Kv8Decode a) {
 
   const int split = blockIdx.x, kvh = blockIdx.y, b = blockIdx.z, G = a.G;
   const int len = min(a.lens[b], a.table_width * kPage);
+  // (asked for together: each would be a trip to memory of its own where it is used)
+  int slot = FUSED && a.slots != nullptr ? a.slots[b] : -1;
+  const int position = FUSED ? a.positions[b] : 0;
   if (len <= 0) {  // an empty row (a graph bucket's slack): zeros
     if (split == 0)
       for (int i = threadIdx.x; i < G * D; i += 256) a.out[act_index(b, kvh * G * D + i, a.out_stride)] = 0;
@@ -151,6 +154,34 @@ __global__ __launch_bounds__(256, 2) void kv8_decode_kernel(const Kv8Decode a) {
 #pragma unroll
     for (int s = 0; s < KS; ++s) qf[s] = *reinterpret_cast<const bf16x8*>(qp + 8 * s);
   }
+  // FUSED: thread's item of the new token's row - 4 rotary pairs of a head: its first four slabs and angles are asked for ahead of the pages
+  constexpr int HALF = D / 2, QP = HALF / 4;
+  const int cols = (a.Hq + 2 * a.Hkv) * D, items = (G + 2) * QP;
+  const long slab = (long)a.B * cols;
+  const float *row = nullptr, *cs = nullptr;
+  f32x4 early[FUSED ? 10 : 1];
+  auto column = [&](int it) {
+    const int h = it / QP;  // h < G: a query head, G: k, G + 1: v
+    return (h < G ? kvh * G + h : h == G ? a.Hq + kvh : a.Hq + a.Hkv + kvh) * D + (it % QP) * 4;
+  };
+  auto ask = [&](int it) {
+    const float* p = row + column(it);
+    const float* q = cs + (it % QP) * 4;
+    early[8] = *reinterpret_cast<const f32x4*>(q);
+    early[9] = *reinterpret_cast<const f32x4*>(q + HALF);
+#pragma unroll
+    for (int z = 0; z < 4; ++z) {
+      const float* pz = p + min(z, a.nslabs - 1) * slab;
+      early[2 * z] = __builtin_nontemporal_load(reinterpret_cast<const f32x4*>(pz));
+      early[2 * z + 1] = __builtin_nontemporal_load(reinterpret_cast<const f32x4*>(pz + HALF));
+    }
+  };
+  if constexpr (FUSED) {
+    row = a.slabs + (long)b * cols;
+    cs = a.cos_sin + (long)min(max(position, 0), a.max_pos - 1) * D;
+    ask(min((int)threadIdx.x, items - 1));
+    __builtin_amdgcn_sched_barrier(0);
+  }
   // Loads return in order and the compiler counts them, so every path through the loop issues the same ones: behind the last step all lanes
   // read one place of the last page.  A buffer's page numbers are asked for behind its data, a turn before they are used.
   Kv8Tiles<D> t0, t1;
@@ -171,47 +202,49 @@ __global__ __launch_bounds__(256, 2) void kv8_decode_kernel(const Kv8Decode a) {
   };
 
   float k_old = 0.f, v_old = 0.f, k_new = 0.f, v_new = 0.f;
-  int slot = -1;
   if constexpr (FUSED) {
-    const int cols = (a.Hq + 2 * a.Hkv) * D;
-    const long slab = (long)a.B * cols;
-    const float* row = a.slabs + (long)b * cols;
-    const float* cs = a.cos_sin + (long)min(max(a.positions[b], 0), a.max_pos - 1) * D;
-    constexpr int HALF = D / 2, QP = HALF / 4;
-    for (int it = threadIdx.x; it < (G + 2) * QP; it += 256) {
-      const int h = it / QP, p = (it - h * QP) * 4;  // h < G: a query head, G: k, G + 1: v
-      const int c = h < G ? (kvh * G + h) * D : (h == G ? (a.Hq + kvh) * D : (a.Hq + a.Hkv + kvh) * D);
+    if (slot >= a.pages * kPage) slot = -1;
+    if (owns_new && slot >= 0 && (slot & (kPage - 1))) {
+      const float* sp = a.scales + ((long)(slot >> 4) * a.Hkv + kvh) * 2;
+      k_old = sp[0];
+      v_old = sp[1];
+    }
+    for (int it = threadIdx.x; it < items; it += 256) {
+      if (it >= 256) ask(it);
+      const int h = it / QP, p = (it % QP) * 4;
       f32x4 x1 = {0.f, 0.f, 0.f, 0.f}, x2 = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll 4
-      for (int z = 0; z < a.nslabs; ++z) {
-        x1 += __builtin_nontemporal_load(reinterpret_cast<const f32x4*>(row + z * slab + c + p));
-        x2 += __builtin_nontemporal_load(reinterpret_cast<const f32x4*>(row + z * slab + c + HALF + p));
+#pragma unroll
+      for (int z = 0; z < 4; ++z)
+        if (z < a.nslabs) {
+          x1 += early[2 * z];
+          x2 += early[2 * z + 1];
+        }
+      for (int z = 4; z < a.nslabs; ++z) {
+        const float* pz = row + column(it) + z * slab;
+        x1 += __builtin_nontemporal_load(reinterpret_cast<const f32x4*>(pz));
+        x2 += __builtin_nontemporal_load(reinterpret_cast<const f32x4*>(pz + HALF));
       }
+      const f32x4 cc = early[8], ss = early[9];
       bf16_t* dst = h < G ? s_q[h] : s_kv[h - G];
+      float lo[4], hi[4];
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         float x = bf2f(f2bf(x1[j])), y = bf2f(f2bf(x2[j]));
         if (h <= G) {  // each product rounded by itself: the page's scale, a threshold on these, is then what elementwise code finds
-          const float c_ = cs[p + j], s_ = cs[HALF + p + j];
-          const float o1 = __fsub_rn(__fmul_rn(x, c_), __fmul_rn(y, s_)), o2 = __fadd_rn(__fmul_rn(y, c_), __fmul_rn(x, s_));
+          const float o1 = __fsub_rn(__fmul_rn(x, cc[j]), __fmul_rn(y, ss[j])), o2 = __fadd_rn(__fmul_rn(y, cc[j]), __fmul_rn(x, ss[j]));
           x = o1;
           y = o2;
         }
-        dst[p + j] = f2bf(x);
-        dst[HALF + p + j] = f2bf(y);
+        lo[j] = x;
+        hi[j] = y;
       }
+      *reinterpret_cast<uint2*>(dst + p) = make_uint2(pack2(lo[0], lo[1]), pack2(lo[2], lo[3]));
+      *reinterpret_cast<uint2*>(dst + HALF + p) = make_uint2(pack2(hi[0], hi[1]), pack2(hi[2], hi[3]));
     }
     __syncthreads();
 #pragma unroll
     for (int s = 0; s < KS; ++s) qf[s] = *reinterpret_cast<const bf16x8*>(&s_q[hc][KD * kg + 8 * s]);
     if (owns_new) {  // uniform: the new token's scales and codes, in every wave; wave 0 leaves what they stand for
-      if (a.slots != nullptr) slot = a.slots[b];
-      if (slot >= a.pages * kPage) slot = -1;
-      if (slot >= 0 && (slot & (kPage - 1))) {
-        const float* sp = a.scales + ((long)(slot >> 4) * a.Hkv + kvh) * 2;
-        k_old = sp[0];
-        v_old = sp[1];
-      }
       // lanes 0..31: 4 dims of k each, 32..63: of v
       const int d = (lane & 31) * 4;
       const uint2 raw = *reinterpret_cast<const uint2*>(&s_kv[lane >> 5][d]);

@@ -33,48 +33,43 @@ struct LogitControls {
   const int* lens;
 };
 
+// 8 logits in a row, as loaded
 template <typename T>
-__device__ __forceinline__ void lc_load(const T* p, float* x, bool vec) {  // 8 in a row
-  if constexpr (sizeof(T) == 2) {
-    if (vec) {
-      unpack8(*reinterpret_cast<const uint4*>(p), x);
+struct LcGroup {
+  static constexpr int N = sizeof(T) / 2;
+  uint4 w[N];
+  __device__ __forceinline__ void load(const T* p) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) w[i] = reinterpret_cast<const uint4*>(p)[i];
+  }
+  __device__ __forceinline__ void get(float* x) const {
+    if constexpr (N == 1) {
+      unpack8(w[0], x);
     } else {
 #pragma unroll
-      for (int j = 0; j < 8; ++j) x[j] = bf2f(p[j]);
-    }
-  } else {
-    if (vec) {
-      const float4 a = *reinterpret_cast<const float4*>(p), b = *reinterpret_cast<const float4*>(p + 4);
-      x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w;
-      x[4] = b.x; x[5] = b.y; x[6] = b.z; x[7] = b.w;
-    } else {
-#pragma unroll
-      for (int j = 0; j < 8; ++j) x[j] = p[j];
+      for (int i = 0; i < 2; ++i) {
+        x[4 * i] = __uint_as_float(w[i].x);
+        x[4 * i + 1] = __uint_as_float(w[i].y);
+        x[4 * i + 2] = __uint_as_float(w[i].z);
+        x[4 * i + 3] = __uint_as_float(w[i].w);
+      }
     }
   }
+};
+
+__device__ __forceinline__ float lc_get(const bf16_t* p) { return bf2f(*p); }
+__device__ __forceinline__ float lc_get(const float* p) { return *p; }
+__device__ __forceinline__ void lc_put(bf16_t* p, float x) { *p = f2bf(x); }
+__device__ __forceinline__ void lc_put(float* p, float x) { *p = x; }
+__device__ __forceinline__ void lc_put8(bf16_t* p, const float* x) { *reinterpret_cast<uint4*>(p) = pack8(x); }
+__device__ __forceinline__ void lc_put8(float* p, const float* x) {
+  *reinterpret_cast<float4*>(p) = make_float4(x[0], x[1], x[2], x[3]);
+  *reinterpret_cast<float4*>(p + 4) = make_float4(x[4], x[5], x[6], x[7]);
 }
 
-template <typename T>
-__device__ __forceinline__ void lc_store(T* p, const float* x, bool vec) {
-  if constexpr (sizeof(T) == 2) {
-    if (vec) {
-      *reinterpret_cast<uint4*>(p) = pack8(x);
-    } else {
-#pragma unroll
-      for (int j = 0; j < 8; ++j) p[j] = f2bf(x[j]);
-    }
-  } else {
-    if (vec) {
-      *reinterpret_cast<float4*>(p) = make_float4(x[0], x[1], x[2], x[3]);
-      *reinterpret_cast<float4*>(p + 4) = make_float4(x[4], x[5], x[6], x[7]);
-    } else {
-#pragma unroll
-      for (int j = 0; j < 8; ++j) p[j] = x[j];
-    }
-  }
-}
+constexpr int kLcGroups = 2;  // of a thread: parts of at most 16384 tokens
 
-// grid (parts, rows); dynamic LDS: `chunk` words (a multiple of 256)
+// grid (parts, rows); dynamic LDS: `chunk` words (a multiple of 256, at most 8 * kLcGroups * kLcThreads)
 template <typename TI, typename TO>
 __global__ __launch_bounds__(kLcThreads) void logit_controls_kernel(TO* out, long out_stride, const TI* in, long in_stride, int V, int chunk,
                                                                     const LogitControls c) {
@@ -86,81 +81,100 @@ __global__ __launch_bounds__(kLcThreads) void logit_controls_kernel(TO* out, lon
   const bool vin = ((uintptr_t)x & 15) == 0, vout = ((uintptr_t)y & 15) == 0;  // uniform; lo is a multiple of 256
   int slot = c.rows[b];
   if (slot >= c.slots) slot = -1;
-  if (slot < 0) {
-    if ((const void*)x == (const void*)y) return;
-    for (int v = lo + tid * 8; v < hi; v += kLcThreads * 8) {
-      if (v + 8 <= hi) {
-        float f[8];
-        lc_load(x + v, f, vin);
-        lc_store(y + v, f, vout);
-      } else {
-        for (int j = v; j < hi; ++j) {
-          if constexpr (sizeof(TI) == 2 && sizeof(TO) == 2) y[j] = x[j];
-          else if constexpr (sizeof(TI) == 2) y[j] = bf2f(x[j]);
-          else y[j] = x[j];
-        }
+  if (slot < 0 && (const void*)x == (const void*)y) return;
+  // What does not hang on one another is asked for together: the history's first 4096 tokens, the slot's numbers, the logits
+  const int* bt = c.table + (long)b * c.table_stride;
+  const int width = c.table_width * 16, t0 = tid * 4;
+  auto history = [&](int t) {
+    const int page = bt[t >> 4];
+    return page >= 0 && page < c.pages ? *reinterpret_cast<const int4*>(c.tokens + (long)page * 16 + (t & 15)) : make_int4(-1, -1, -1, -1);
+  };
+  int4 first = make_int4(-1, -1, -1, -1);
+  if (t0 < width) first = history(t0);
+  const int len = min(c.lens[b], width);
+  int prompt = 0, entry = -1;
+  float rep = 1.f, pres = 0.f, freq = 0.f;
+  bool masked = false;
+  const uint32_t* mask = c.masks;
+  const int* bi = c.bias_ids;
+  if (slot >= 0) {
+    prompt = c.info[2 * slot];
+    masked = c.info[2 * slot + 1] != 0;
+    rep = c.params[3 * slot];
+    pres = c.params[3 * slot + 1];
+    freq = c.params[3 * slot + 2];
+    mask += (long)slot * c.words;
+    bi += (long)slot * c.n_bias;
+    if (tid < c.n_bias) entry = bi[tid];
+  }
+  LcGroup<TI> g[kLcGroups];
+#pragma unroll
+  for (int i = 0; i < kLcGroups; ++i) {
+    const int v = lo + (i * kLcThreads + tid) * 8;
+    if (vin && v + 8 <= hi) g[i].load(x + v);
+  }
+  if (slot >= 0) {
+    for (int i = tid * 4; i < chunk; i += kLcThreads * 4) *reinterpret_cast<uint4*>(s_word + i) = make_uint4(0, 0, 0, 0);
+    __syncthreads();
+    // bias entries beside the history: of several with one token the first counts, the one with the largest n_bias - j
+    for (int j = tid; j < c.n_bias; j += kLcThreads) {
+      const int v = j == tid ? entry : bi[j];
+      if (v < lo || v >= hi) continue;
+      const uint32_t mine = (uint32_t)(c.n_bias - j);
+      uint32_t* p = &s_word[v - lo];
+      uint32_t had = *p;
+      while ((had >> kLcBias) < mine) {  // ends: another's write either leaves a larger number or the compare succeeds
+        const uint32_t now = atomicCAS(p, had, (had & (kLcPrompt | kLcCount)) | mine << kLcBias);
+        if (now == had) break;
+        had = now;
       }
     }
-    return;
-  }
-  for (int i = tid * 4; i < chunk; i += kLcThreads * 4) *reinterpret_cast<uint4*>(s_word + i) = make_uint4(0, 0, 0, 0);
-  __syncthreads();
-  // the bias entries first: of several with one token the first counts, the largest n_bias - j
-  const int* bi = c.bias_ids + (long)slot * c.n_bias;
-  for (int j = tid; j < c.n_bias; j += kLcThreads) {
-    const int v = bi[j];
-    if (v >= lo && v < hi) atomicMax(&s_word[v - lo], (uint32_t)(c.n_bias - j) << kLcBias);
-  }
-  __syncthreads();
-  const int len = min(c.lens[b], c.table_width * 16), prompt = c.info[2 * slot];
-  const int* bt = c.table + (long)b * c.table_stride;
-  for (int t = tid * 4; t < len; t += kLcThreads * 4) {
-    const int page = bt[t >> 4];
-    if (page < 0 || page >= c.pages) continue;
-    const int4 q = *reinterpret_cast<const int4*>(c.tokens + (long)page * 16 + (t & 15));
-    const int id[4] = {q.x, q.y, q.z, q.w};
+    for (int t = t0; t < len; t += kLcThreads * 4) {
+      const int4 q = t == t0 ? first : history(t);
+      const int id[4] = {q.x, q.y, q.z, q.w};
 #pragma unroll
-    for (int j = 0; j < 4; ++j)
-      if (t + j < len && id[j] >= lo && id[j] < hi) {
-        if (t + j < prompt) atomicOr(&s_word[id[j] - lo], kLcPrompt);
-        else atomicAdd(&s_word[id[j] - lo], 1u);
-      }
+      for (int j = 0; j < 4; ++j)
+        if (t + j < len && id[j] >= lo && id[j] < hi) {
+          if (t + j < prompt) atomicOr(&s_word[id[j] - lo], kLcPrompt);
+          else atomicAdd(&s_word[id[j] - lo], 1u);
+        }
+    }
+    __syncthreads();
   }
-  __syncthreads();
-  const float rep = c.params[3 * slot], pres = c.params[3 * slot + 1], freq = c.params[3 * slot + 2];
-  const bool masked = c.info[2 * slot + 1] != 0;
-  const uint32_t* mask = c.masks + (long)slot * c.words;
-  const float* bv = c.bias_vals + (long)slot * c.n_bias;
+  const float* bv = c.bias_vals + (long)max(slot, 0) * c.n_bias;
+  const float inv = 1.f / rep;  // (a quotient for each token of a row's frequent ones is what the slowest workgroups would spend their time on)
   auto one = [&](float f, uint32_t w) {
     const float count = (float)(w & kLcCount);
-    if (w & (kLcPrompt | kLcCount)) f = f > 0.f ? f / rep : f * rep;
+    if (w & (kLcPrompt | kLcCount)) f *= f > 0.f ? inv : rep;
     if (w & kLcCount) f = f - freq * count - pres;
     if (w >> kLcBias) f += bv[c.n_bias - (int)(w >> kLcBias)];
     return f;
   };
-  for (int v = lo + tid * 8; v < hi; v += kLcThreads * 8) {
-    const uint32_t ok = masked ? mask[v >> 5] >> (v & 31) : 0xffu;  // v is a multiple of 8
-    if (v + 8 <= hi) {
-      float f[8];
-      lc_load(x + v, f, vin);
-      const uint4 a = *reinterpret_cast<const uint4*>(s_word + v - lo), d = *reinterpret_cast<const uint4*>(s_word + v - lo + 4);
-      const uint32_t w[8] = {a.x, a.y, a.z, a.w, d.x, d.y, d.z, d.w};
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        if (w[j]) f[j] = one(f[j], w[j]);
-        if (!((ok >> j) & 1)) f[j] = -INFINITY;
+  for (int i = 0; i < kLcGroups; ++i) {
+    const int v = lo + (i * kLcThreads + tid) * 8;
+    if (v >= hi) break;
+    const uint32_t ok = masked ? mask[v >> 5] >> (v & 31) : 0xffu;  // v is a multiple of 8
+    if (vin && vout && v + 8 <= hi) {
+      float f[8];
+      g[i].get(f);
+      if (slot >= 0) {
+        const uint4 p = *reinterpret_cast<const uint4*>(s_word + v - lo), q = *reinterpret_cast<const uint4*>(s_word + v - lo + 4);
+        const uint32_t w[8] = {p.x, p.y, p.z, p.w, q.x, q.y, q.z, q.w};
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          if (w[j]) f[j] = one(f[j], w[j]);
+          if (!((ok >> j) & 1)) f[j] = -INFINITY;
+        }
       }
-      lc_store(y + v, f, vout);
-    } else {
-      for (int j = v; j < hi; ++j) {
-        float f;
-        if constexpr (sizeof(TI) == 2) f = bf2f(x[j]);
-        else f = x[j];
-        const uint32_t w = s_word[j - lo];
+      lc_put8(y + v, f);
+    } else {  // a row that does not start at 16 bytes, or its end
+      for (int j = v; j < min(v + 8, hi); ++j) {
+        float f = lc_get(x + j);
+        const uint32_t w = slot >= 0 ? s_word[j - lo] : 0u;
         if (w) f = one(f, w);
         if (!((ok >> (j - v)) & 1)) f = -INFINITY;
-        if constexpr (sizeof(TO) == 2) y[j] = f2bf(f);
-        else y[j] = f;
+        lc_put(y + j, f);
       }
     }
   }
