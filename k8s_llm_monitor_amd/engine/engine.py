@@ -27,6 +27,7 @@ from typing import Optional, Union
 import torch
 
 from ..models.config import ModelConfig, get_config
+from ..ops.logits import check_controls
 from ..models.registry import build_model, config_from_dir
 from ..parallel.state import ParallelState, get_state, serving_timeouts
 from ..parallel.step_bus import KIND_DECODE, KIND_PICKLE, KIND_STOP, bus_slot_bytes, decode_message, make_step_bus
@@ -51,6 +52,12 @@ class EngineConfig:
     # and the prefill backlog exceeds one step; 0 = always mix.  K8SLLM_DECODE_STALL_STEPS
     max_decode_stall_steps: int = field(default_factory=lambda: int(os.environ.get("K8SLLM_DECODE_STALL_STEPS", "8")))
     kv_cache_gb: float = 32.0
+    # "auto": the cache holds the compute dtype; "fp8": e4m3 codes with a scale for each 16-token block and kv head
+    # (ops/kv8.py) - half the memory and decode traffic, twice the tokens of kv_cache_gb
+    kv_cache_dtype: str = "auto"
+    # requests may have penalties, biases and allowed tokens (SamplingParams); two small launches a step
+    logit_controls: bool = False
+    max_logit_bias: int = 300  # biased tokens a request
     num_blocks: Optional[int] = None
     use_graphs: bool = True
     seed: int = 0
@@ -101,11 +108,14 @@ class LLMEngine:
         if cfg.model_overrides:
             mc = mc.replace(**cfg.model_overrides)
         self.model_cfg = mc
+        if cfg.logit_controls and self.ps.tp_size > 1:
+            raise ValueError("logit_controls: tensor parallelism is not supported (the workers do not get the requests' controls)")
         t0 = time.perf_counter()
         self.model = build_model(mc, device=self.device, dtype=getattr(torch, cfg.dtype), seed=cfg.seed,
                                  pstate=self.ps, weights=cfg.weights)
         self.runner = ModelRunner(self.model, RunnerConfig(
             max_num_seqs=cfg.max_num_seqs, max_model_len=cfg.max_model_len, kv_cache_gb=cfg.kv_cache_gb,
+            kv_cache_dtype=cfg.kv_cache_dtype, logit_controls=cfg.logit_controls, max_logit_bias=cfg.max_logit_bias,
             num_blocks=cfg.num_blocks, use_graphs=cfg.use_graphs, seed=cfg.seed, keep_logits=cfg.keep_logits,
             sample=cfg.sample))
         self.blocks = BlockManager(self.runner.num_blocks, prefix_caching=cfg.prefix_caching,
@@ -162,6 +172,8 @@ class LLMEngine:
         """``deadline`` (time.perf_counter clock): the sequence stops with finish_reason "deadline"
         at the first step resolved after it - an answer truncated to what fits the caller's time
         budget instead of work the caller has stopped waiting for."""
+        if params is not None and params.controlled:
+            self._check_controls(params)
         ids = self.tokenizer.encode(prompt) if isinstance(prompt, str) else list(prompt)
         limit = self.runner.max_len - 1
         if len(ids) > limit - 1:  # keep room for at least one generated token; trim the middle
@@ -175,6 +187,18 @@ class LLMEngine:
         self.counters["requests"] += 1
         self.counters["prompt_tokens"] += len(ids)
         return seq
+
+    def _check_controls(self, p: SamplingParams) -> None:
+        """ValueError for controls that this engine does not take."""
+        if not self.cfg.logit_controls:
+            raise ValueError("penalties, logit_bias and allowed_token_ids need an engine with logit_controls")
+        V, bias = self.model_cfg.vocab_size, p.logit_bias or {}
+        check_controls(p.repetition_penalty, p.presence_penalty, p.frequency_penalty, bias)
+        if len(bias) > self.cfg.max_logit_bias:
+            raise ValueError(f"logit_bias: at most {self.cfg.max_logit_bias} tokens, are {len(bias)}")
+        ids = list(bias) + list(p.allowed_token_ids or ())
+        if any(int(t) != t or not 0 <= t < V for t in ids) or (p.allowed_token_ids is not None and not len(p.allowed_token_ids)):
+            raise ValueError(f"logit_bias and allowed_token_ids: token ids below {V}, at least one allowed")
 
     def has_work(self) -> bool:
         return self.sched.has_work() or self._inflight is not None or self._pf_inflight is not None

@@ -23,7 +23,7 @@ import torch
 
 from .. import ops
 from ..models.llama import AttnMeta, CausalLM, PageList
-from .sequence import Sequence
+from .sequence import Sequence, SeqStatus
 
 BLOCK_SIZE = 16
 DEFAULT_BUCKETS = (1, 2, 4, 8, 16, 24, 32, 40, 48, 56, 64, 80, 96, 112, 128, 160, 192, 224, 256)
@@ -34,6 +34,10 @@ class RunnerConfig:
     max_num_seqs: int = 64
     max_model_len: int = 8192
     kv_cache_gb: float = 16.0  # <= 0: max_num_seqs x max_model_len worth of blocks
+    kv_cache_dtype: str = "auto"  # "fp8": pages of e4m3 codes (ops/kv8.py)
+    # penalties, biases and masks of SamplingParams; the pages of token ids that they need are kept for every sequence
+    logit_controls: bool = False
+    max_logit_bias: int = 300
     num_blocks: Optional[int] = None  # overrides kv_cache_gb
     use_graphs: bool = True
     seed: int = 0
@@ -56,12 +60,19 @@ class ModelRunner:
         # layer-list models (models/hybrid.py) describe their own per-run caches: paged K / V for
         # attention runs, per-sequence state slots for recurrent runs
         self.hybrid = hasattr(model, "new_cache")
+        if cfg.kv_cache_dtype not in ("auto", "fp8"):
+            raise ValueError(f"kv_cache_dtype {cfg.kv_cache_dtype!r}: auto or fp8")
+        self.kv8 = cfg.kv_cache_dtype == "fp8"
+        if self.kv8 and self.hybrid:
+            raise ValueError("kv_cache_dtype fp8: layer-list models keep caches of their own")
         if self.hybrid:
             per_block, per_slot = model.cache_bytes()
             per_block = max(1, per_block)
         else:
             L, hkv, D = c.n_layers, model.hkv, model.D
-            per_block = 2 * L * hkv * D * BLOCK_SIZE * 2  # bytes (K + V, bf16)
+            if self.kv8 and (D not in (64, 128) or model.hq // hkv > 16):
+                raise ValueError(f"kv_cache_dtype fp8: head size 64 or 128 and at most 16 query heads a kv head, are {D} and {model.hq // hkv}")
+            per_block = L * ops.kv8_block_bytes(hkv, D) if self.kv8 else 2 * L * hkv * D * BLOCK_SIZE * 2  # bytes (K + V, bf16)
         if cfg.num_blocks:
             nb = cfg.num_blocks
         elif cfg.kv_cache_gb <= 0:  # auto: every admitted sequence can reach max_len (+ one spare block)
@@ -73,6 +84,10 @@ class ModelRunner:
         if self.hybrid:
             self.k_cache = self.v_cache = None
             self.kv = model.new_cache(nb, max(1, self.num_state_slots))
+        elif self.kv8:
+            cache = ops.kv8_cache(nb, hkv, D, device=self.device, layers=L)
+            self.k_cache, self.v_cache = cache.k, cache.v
+            self.kv = [cache.layer(i) for i in range(L)]
         else:
             self.k_cache = torch.zeros(L, nb, hkv, D // 8, BLOCK_SIZE, 8, dtype=model.dtype, device=self.device)
             self.v_cache = torch.zeros(L, nb, hkv, D, BLOCK_SIZE, dtype=model.dtype, device=self.device)
@@ -93,6 +108,17 @@ class ModelRunner:
         self.d_logits = None  # [B, vocab] fp32, the last decode step's logits (cfg.keep_logits)
         self.last_logits = None
         self.d_topp.fill_(1.0)
+        # controls of logits: a slot for each running sequence that has any, rows of a step name theirs (-1: none)
+        self.controls = None
+        if cfg.logit_controls:
+            self.controls = ops.logit_controls(B, c.vocab_size, cfg.max_logit_bias, device=dev)
+            self.token_cache = torch.zeros(nb, BLOCK_SIZE, dtype=torch.int32, device=dev)
+            self.d_ctl = torch.full((B,), -1, dtype=torch.int32, device=dev)
+            self.h_ctl = [torch.full((B,), -1, dtype=torch.int32, pin_memory=self.is_gpu) for _ in range(2)]
+            # 32 bits: penalties smaller than a bf16 step of the logits count
+            self.d_ctl_logits = torch.empty(B, c.vocab_size, dtype=torch.float32, device=dev)
+            self._ctl: dict = {}  # sequence id -> (slot, sequence)
+            self._ctl_free = list(range(B))
         self.rng = torch.tensor([cfg.seed, 0], dtype=torch.int64, device=dev)
         self.d_out = torch.zeros(B, dtype=torch.int32, device=dev)
         self.decode_ws = ops.decode_workspace(B, model.hq, D, self.max_blocks_per_seq * BLOCK_SIZE, dev, model.hkv) \
@@ -145,6 +171,25 @@ class ModelRunner:
     def _sample(self, logits: torch.Tensor, temp, topk, topp, out=None) -> torch.Tensor:
         # fresh numbers next step: the counter advances inside the sampling kernel (also in a graph)
         return ops.sample(logits, temp, topk, topp, self.rng, out=out, advance=True)
+
+    def _control_slot(self, s) -> int:
+        """The slot of a sequence's controls (filled when it gets one), -1 if it has none.  Slots of sequences that run no more are
+        taken back when none is free; a preempted sequence gets a new one."""
+        if self.controls is None or not s.params.controlled:
+            return -1
+        hit = self._ctl.get(s.seq_id)
+        if hit is not None:
+            return hit[0]
+        if not self._ctl_free:
+            for k, (slot, q) in list(self._ctl.items()):
+                if q.status != SeqStatus.RUNNING:
+                    del self._ctl[k]
+                    self._ctl_free.append(slot)
+        slot, p = self._ctl_free.pop(), s.params
+        self.controls.set(slot, len(s.prompt_ids), p.repetition_penalty, p.presence_penalty, p.frequency_penalty, p.logit_bias,
+                          p.allowed_token_ids)
+        self._ctl[s.seq_id] = slot, s
+        return slot
 
     # --------------------------------------------------------------------- prefill
     def prefill(self, seqs: list[Sequence], decode: Optional[list] = None) -> list[int]:
@@ -222,6 +267,12 @@ class ModelRunner:
             sizes.update(mcu=len(seqs) + 2, mqs=nq, mst=nq, mlidx=len(seqs))
         for w, (_, _, ends) in seen.items():
             sizes[f"pgl{w}"], sizes[f"pgb{w}"] = ends[-1], len(seqs) * W
+        ctl = [self._control_slot(s) for s in rows] if self.controls is not None and logit_rows is None else []
+        if any(c >= 0 for c in ctl):  # the rows' histories: every row's pages and tokens
+            Wc = max(len(s.block_table) for s in rows)
+            sizes.update(crow=R, clen=R, cbt=R * Wc)
+        else:
+            ctl = []
         off, o = {}, 0
         for k, n in sizes.items():
             off[k] = o
@@ -260,6 +311,13 @@ class ModelRunner:
             v["gctx"][nd:] = starts
             v["gslot"][:] = [getattr(q, "state_slot", -1) for q in rows]
             v["cend"][:] = [c + n for c, n in zip(starts, lens)]
+        if ctl:
+            v["crow"][:] = ctl
+            v["clen"][:] = [q.num_tokens for q in decode] + [c + n for c, n in zip(starts, lens)]
+            cbt = v["cbt"].reshape(R, Wc)
+            cbt[:] = 0
+            for i, s in enumerate(rows):
+                cbt[i, : len(s.block_table)] = s.block_table
         v["temp"].view(np.float32)[:] = [s.params.temperature for s in rows]
         v["topk"][:] = [s.params.top_k for s in rows]
         v["topp"].view(np.float32)[:] = [s.params.top_p for s in rows]
@@ -333,9 +391,14 @@ class ModelRunner:
         # tokens attended from the paged cache instead of recomputed (prefix hits + earlier chunks)
         self.n_steps["prefill_context_tokens"] = self.n_steps.get("prefill_context_tokens", 0) + sum(starts)
         self.n_steps["prefill_tokens"] = self.n_steps.get("prefill_tokens", 0) + T
+        if self.controls is not None:
+            ops.cache_tokens(self.token_cache, dv["ids"], dv["slots"])
         logits = self.model.forward(dv["ids"], meta, self.kv)
         if self.cfg.keep_logits:
             self.last_logits = logits
+        if ctl:
+            logits = ops.control_logits(logits, self.controls, dv["crow"], self.token_cache, dv["cbt"].view(R, Wc), dv["clen"],
+                                        out=torch.empty(logits.shape, dtype=torch.float32, device=dev))
         self.n_steps["prefill"] += 1
         if logit_rows is not None:
             return DecodeHandle(nl, None, [], logits=logits)
@@ -370,6 +433,11 @@ class ModelRunner:
                 self.d_logits = torch.zeros(self.B, logits.shape[1], dtype=torch.float32, device=self.device)
             self.d_logits[:b].copy_(logits)
             self.last_logits = self.d_logits[:b]
+        if self.controls is not None:  # (d_out still holds the tokens of the step before)
+            ops.cache_tokens(self.token_cache, self.d_ids[:b], self.d_slots[:b], self.d_src[:b], self.d_out)
+            if self.cfg.sample:
+                logits = ops.control_logits(logits, self.controls, self.d_ctl[:b], self.token_cache, self.d_bt[:b], self.d_lens[:b],
+                                            out=self.d_ctl_logits[:b])
         if self.cfg.sample:
             self._sample(logits, self.d_temp[:b], self.d_topk[:b], self.d_topp[:b], out=self.d_out[:b])
 
@@ -396,7 +464,7 @@ class ModelRunner:
                 g = torch.cuda.CUDAGraph()
                 with torch.cuda.graph(g, pool=self.graph_pool):
                     if st is not None:
-                        self.d_all[:n_el].copy_(st.h_all[:n_el], non_blocking=True)
+                        self._copy_staged(st, b, n_el)
                     self._decode_body(b)
                 gs.append(g)
             self.graphs[b] = gs
@@ -437,6 +505,10 @@ class ModelRunner:
             temp[i] = p.temperature
             topk[i] = p.top_k
             topp[i] = p.top_p
+        if self.controls is not None:
+            c = self.h_ctl[st.idx].numpy()
+            c[:n] = [self._control_slot(s) for s in seqs]
+            c[n:b] = -1
         if b > n:
             ids[n:b] = 0
             src[n:b] = -1
@@ -464,7 +536,7 @@ class ModelRunner:
         if gs is not None and self.graph_h2d:
             gs[st.idx].replay()  # its first node copies this staging buffer (n_el = the bucket's prefix)
         else:
-            self.d_all[:n_el].copy_(st.h_all[:n_el], non_blocking=True)
+            self._copy_staged(st, b, n_el)
             if gs is not None:
                 gs[0].replay()
             else:
@@ -479,6 +551,11 @@ class ModelRunner:
         h[:n].copy_(self.d_out[:n], non_blocking=True)
         ev, prev = self._chain_event()
         return DecodeHandle(n, ev, h, prev)
+
+    def _copy_staged(self, st: "_Staging", b: int, n_el: int) -> None:
+        self.d_all[:n_el].copy_(st.h_all[:n_el], non_blocking=True)
+        if self.controls is not None:
+            self.d_ctl[:b].copy_(self.h_ctl[st.idx][:b], non_blocking=True)
 
     def _chain_event(self) -> tuple:
         """Record the end-of-step event (timing-enabled) and return it with the previous launched
@@ -508,6 +585,8 @@ class ModelRunner:
             kv = sum(size(c) for c in self.kv)
         else:
             kv = (self.k_cache.numel() + self.v_cache.numel()) * self.k_cache.element_size()
+            if self.kv8:
+                kv += sum(c.scales.numel() * 4 for c in self.kv)
         return {"kv_cache_bytes": kv, "kv_blocks": self.num_blocks, "block_size": BLOCK_SIZE,
                 "max_model_len": self.max_len, "graph_buckets": sorted(self.graphs)}
 

@@ -19,6 +19,17 @@ class SamplingParams:
     top_p: float = 1.0
     ignore_eos: bool = False
     stop_token_ids: tuple = ()
+    # controls of the logits ahead of sampling (ops/logits.py; EngineConfig.logit_controls)
+    repetition_penalty: float = 1.0  # of tokens in the prompt or the answer: x > 0 ? x / r : x * r
+    presence_penalty: float = 0.0  # off tokens that the answer has
+    frequency_penalty: float = 0.0  # off them for each time that it has them
+    logit_bias: Optional[dict] = None  # token id -> addend
+    allowed_token_ids: Optional[tuple] = None  # only these are sampled (None: all)
+
+    @property
+    def controlled(self) -> bool:
+        return (self.repetition_penalty != 1.0 or self.presence_penalty != 0.0 or self.frequency_penalty != 0.0
+                or bool(self.logit_bias) or self.allowed_token_ids is not None)
 
 
 class SeqStatus(enum.Enum):

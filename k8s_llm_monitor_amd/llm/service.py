@@ -69,6 +69,8 @@ class LocalEngineBackend:
         eng = service.engine
         mml = getattr(getattr(eng, "cfg", None), "max_model_len", None) or (1 << 30)
         self.max_len = min(int(mml), int(eng.model_cfg.max_position))  # the engine's per-sequence cap
+        # whether generate() takes ``controls`` (llm.logit_controls)
+        self.takes_controls = bool(getattr(getattr(eng, "cfg", None), "logit_controls", False))
 
     def max_prompt_tokens(self, max_tokens: Optional[int] = None) -> int:
         """Prompt tokens that still leave room for ``max_tokens`` answer tokens (preamble included);
@@ -81,13 +83,14 @@ class LocalEngineBackend:
 
     def generate(self, prompt: str, max_tokens: Optional[int] = None, temperature: Optional[float] = None,
                  request_id: Optional[str] = None, ignore_eos: bool = False,
-                 top_p: Optional[float] = None) -> GenResult:
+                 top_p: Optional[float] = None, controls: Optional[dict] = None) -> GenResult:
+        """``controls``: SamplingParams' presence_penalty, frequency_penalty, repetition_penalty and logit_bias."""
         from ..engine import SamplingParams
 
         d = self.default
         p = SamplingParams(max_tokens=max_tokens or d.max_tokens,
                            temperature=d.temperature if temperature is None else temperature,
-                           top_k=d.top_k, top_p=d.top_p if top_p is None else top_p, ignore_eos=ignore_eos)
+                           top_k=d.top_k, top_p=d.top_p if top_p is None else top_p, ignore_eos=ignore_eos, **(controls or {}))
         budget = self.answer_budget_s
         fut = self.svc.submit(P.SYSTEM_PREAMBLE + prompt, p, request_id,
                               deadline=time.perf_counter() + budget if budget else None)

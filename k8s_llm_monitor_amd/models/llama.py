@@ -309,7 +309,8 @@ class CausalLM:
         or fragment-packed with ``rows`` valid rows), reduced inside rope_and_cache; the attention
         output is then written fragment-packed for the o_proj skinny GEMM."""
         c = self.cfg
-        k_cache, v_cache = kv if kv is not None else (None, None)
+        kv8 = kv if isinstance(kv, ops.KV8) else None  # pages of e4m3 codes (RunnerConfig.kv_cache_dtype)
+        k_cache, v_cache = kv[:2] if kv is not None else (None, None)
         partial, ns = None, 0
         roped = False  # q / k already rotated by the qkv GEMM's epilogue
         T = rows if rows is not None else x.shape[0]
@@ -320,6 +321,10 @@ class CausalLM:
             if self._attn_rope and not meta.is_prefill and k_cache is not None and c.arch == "llama":
                 # the attention kernel reduces the slabs, applies RoPE and writes the new k / v
                 out = ops.packed_empty(T, self.hq * self.D, self.dtype, self.device)
+                if kv8 is not None:
+                    return ops.paged_decode_fused_kv8(ws, ns, meta.positions, cs, meta.slot_mapping, kv8, meta.block_tables,
+                                                      meta.seq_lens, self.hq, self.hkv, self.D, self.scale,
+                                                      workspace=meta.decode_ws, out=out)
                 return ops.paged_decode_fused(ws, ns, meta.positions, cs, meta.slot_mapping, k_cache, v_cache,
                                               meta.block_tables, meta.seq_lens, self.hq, self.hkv, self.D, self.scale,
                                               workspace=meta.decode_ws, out=out)
@@ -333,28 +338,45 @@ class CausalLM:
                                             rowscale=rowscale)
         else:
             qkv = ops.prefill_linear(x, L["wqkv"])
-        ops.rope_and_cache(qkv, meta.positions, cs, k_cache, v_cache,
-                           meta.slot_mapping if k_cache is not None else None, self.hq, self.hkv, self.D,
-                           apply_rope=c.arch == "llama" and not roped, partial=partial, nslabs=ns)
+        rope = c.arch == "llama" and not roped
+        if kv8 is not None:
+            ops.rope_and_cache_kv8(qkv, meta.positions, cs, kv8, meta.slot_mapping, self.hq, self.hkv, self.D, apply_rope=rope,
+                                   partial=partial, nslabs=ns)
+        else:
+            ops.rope_and_cache(qkv, meta.positions, cs, k_cache, v_cache,
+                               meta.slot_mapping if k_cache is not None else None, self.hq, self.hkv, self.D,
+                               apply_rope=rope, partial=partial, nslabs=ns)
         if meta.is_prefill:
             qb = (meta.qb_seq, meta.qb_start) if meta.qb_seq is not None else None
             paged = None
             if meta.ctx_start is not None:  # some prompts start with cached prefix blocks
                 paged = (meta.ctx_start, k_cache, v_cache, meta.block_tables)
+
+            def prefill(rows, out=None):
+                if kv8 is not None and paged is not None:  # (whole prompts attend their own rows, which are at hand in full)
+                    return ops.flash_prefill_kv8(rows, meta.cu_seqlens, meta.ctx_start, kv8, meta.block_tables, self.hq, self.hkv,
+                                                 self.D, self.scale, qblocks=qb, out=out)
+                return ops.flash_prefill(rows, meta.cu_seqlens, self.hq, self.hkv, self.D, self.scale, qblocks=qb,
+                                         paged=paged, out=out)
             nd = meta.num_decode
             if nd == 0:
-                return ops.flash_prefill(qkv, meta.cu_seqlens, self.hq, self.hkv, self.D, self.scale, qblocks=qb,
-                                         paged=paged)
+                return prefill(qkv)
             # mixed step: decode rows through paged_decode, prefill rows through flash prefill
             o = torch.empty(qkv.shape[0], self.hq * self.D, dtype=qkv.dtype, device=qkv.device)
-            ops.paged_decode(qkv[:nd], k_cache, v_cache, meta.dec_block_tables, meta.dec_seq_lens, self.hq,
-                             self.hkv, self.D, self.scale, workspace=meta.decode_ws, out=o[:nd])
-            op = ops.flash_prefill(qkv[nd:], meta.cu_seqlens, self.hq, self.hkv, self.D, self.scale, qblocks=qb,
-                                   paged=paged, out=o[nd:])
+            if kv8 is not None:
+                ops.paged_decode_kv8(qkv[:nd], kv8, meta.dec_block_tables, meta.dec_seq_lens, self.hq, self.hkv, self.D, self.scale,
+                                     workspace=meta.decode_ws, out=o[:nd])
+            else:
+                ops.paged_decode(qkv[:nd], k_cache, v_cache, meta.dec_block_tables, meta.dec_seq_lens, self.hq,
+                                 self.hkv, self.D, self.scale, workspace=meta.decode_ws, out=o[:nd])
+            op = prefill(qkv[nd:], out=o[nd:])
             if op.data_ptr() != o[nd:].data_ptr():  # CPU reference paths return a fresh tensor
                 o[nd:] = op
         else:
             out = ops.packed_empty(T, self.hq * self.D, self.dtype, self.device) if slabs is not None else None
+            if kv8 is not None:
+                return ops.paged_decode_kv8(qkv, kv8, meta.block_tables, meta.seq_lens, self.hq, self.hkv, self.D, self.scale,
+                                            workspace=meta.decode_ws, out=out)
             o = ops.paged_decode(qkv, k_cache, v_cache, meta.block_tables, meta.seq_lens, self.hq, self.hkv,
                                  self.D, self.scale, workspace=meta.decode_ws, out=out)
         return o

@@ -67,7 +67,8 @@ def engine_config(cfg: Config):
     from ..engine import EngineConfig
 
     return EngineConfig(model=cfg.llm.model, max_num_seqs=cfg.llm.max_batch, max_model_len=cfg.llm.max_model_len,
-                        kv_cache_gb=cfg.llm.kv_cache_gb, use_graphs=cfg.llm.use_graphs, seed=cfg.llm.seed,
+                        kv_cache_gb=cfg.llm.kv_cache_gb, kv_cache_dtype=cfg.llm.kv_cache_dtype,
+                        logit_controls=cfg.llm.logit_controls, use_graphs=cfg.llm.use_graphs, seed=cfg.llm.seed,
                         tp_size=cfg.llm.tp_size, dtype=torch_dtype_name(cfg.llm.dtype),
                         max_prefill_tokens=cfg.llm.max_prefill_tokens, chunked_prefill=cfg.llm.chunked_prefill,
                         prefix_caching=cfg.llm.prefix_caching, weights=cfg.llm.weights or None)

@@ -8,7 +8,7 @@ keys are ignored.  A missing file is an error, like ``viper.ReadInConfig``.
 
 New engine knobs live under ``llm`` next to the reference's keys: ``provider: local-rocm`` selects
 the in-process MI355X engine (``openai`` keeps the reference's remote semantics: no local model),
-plus ``tp_size``, ``dp_replicas``, ``max_batch``, ``kv_cache_gb``, ``max_model_len``, ``dtype``,
+plus ``tp_size``, ``dp_replicas``, ``max_batch``, ``kv_cache_gb``, ``kv_cache_dtype``, ``logit_controls``, ``max_model_len``, ``dtype``,
 ``seed``, ``use_graphs``.
 """
 from __future__ import annotations
@@ -50,6 +50,8 @@ class LLMConfig:
     dp_replicas: int = 1
     max_batch: int = 64
     kv_cache_gb: float = 32.0
+    kv_cache_dtype: str = "auto"  # "fp8": 8-bit KV cache with a scale for each block and head
+    logit_controls: bool = False  # requests may have penalties, logit_bias and allowed tokens
     max_model_len: int = 8192
     dtype: str = "bf16"
     seed: int = 0

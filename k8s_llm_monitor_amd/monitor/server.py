@@ -445,13 +445,20 @@ class MonitorApp:
         top_p = d.get("top_p")
         top_p = float(top_p) if isinstance(top_p, (int, float)) and 0 < top_p <= 1 else None
         backend = self.analysis.backend
+        # penalties and biases are for backends that have them (llm.logit_controls); others go without, as ever
+        controls = _chat_controls(d) if getattr(backend, "takes_controls", False) else {}
         try:
             prompt = self.analysis.fit_chat(parts, mt)
-            g = self._bounded(lambda: backend.generate(prompt, max_tokens=mt, temperature=temp, top_p=top_p))
+            more = {"controls": controls} if controls else {}
+            g = self._bounded(lambda: backend.generate(prompt, max_tokens=mt, temperature=temp, top_p=top_p, **more))
         except _BUSY as e:
             return self._busy_reply(e)
         except FutTimeout:
             raise http_error(504, "answer not ready within the server write timeout")
+        except ValueError as e:
+            if controls:  # refused by the engine: a token outside the vocabulary, too many
+                raise http_error(400, str(e))
+            raise http_error(500, f"{type(e).__name__}: {e}")
         except Exception as e:  # noqa: BLE001
             raise http_error(500, f"{type(e).__name__}: {e}")
         pt, ct = g.get("prompt_tokens"), g.get("completion_tokens")
@@ -583,6 +590,23 @@ def prometheus_text(app: "MonitorApp") -> str:
 def _only(method: str, allowed: str) -> None:
     if method != allowed:
         raise http_error(405, "Method not allowed")
+
+
+def _chat_controls(d: dict) -> dict:
+    """SamplingParams' fields from a chat request's presence_penalty, frequency_penalty, repetition_penalty and logit_bias (token ids as JSON
+    keys); 400 for values of another type."""
+    c = {}
+    for k in ("presence_penalty", "frequency_penalty", "repetition_penalty"):
+        if d.get(k) is not None:
+            if not isinstance(d[k], (int, float)) or isinstance(d[k], bool):
+                raise http_error(400, f"{k} must be a number")
+            c[k] = float(d[k])
+    if d.get("logit_bias"):
+        try:
+            c["logit_bias"] = {int(t): float(x) for t, x in d["logit_bias"].items()}
+        except (AttributeError, TypeError, ValueError):
+            raise http_error(400, "logit_bias must map token ids to numbers") from None
+    return c
 
 
 def _decode_object(body: bytes) -> Optional[dict]:

@@ -1,0 +1,234 @@
+"""The engine over an 8-bit KV cache, and with controls of logits."""
+import json
+
+import pytest
+import torch
+
+from k8s_llm_monitor_amd.engine import EngineConfig, LLMEngine, SamplingParams
+from k8s_llm_monitor_amd.engine.engine import EngineService
+
+DEVICES = ["cpu", pytest.param("cuda", marks=pytest.mark.gpu)]
+GREEDY = dict(temperature=0.0, ignore_eos=True)
+
+
+def engine(dev, **kw):
+    kw = {"model": "llama-tiny-d128", "max_num_seqs": 4, "max_model_len": 512, "num_blocks": 128, **kw}
+    kw.setdefault("dtype", "bfloat16" if dev == "cuda" else "float32")
+    e = LLMEngine(EngineConfig(**kw), device="cuda:0" if dev == "cuda" else "cpu")
+    if dev == "cuda":
+        e.warmup()
+    return e
+
+
+def prompt(n, seed):
+    return torch.randint(3, 250, (n,), generator=torch.Generator().manual_seed(seed)).tolist()
+
+
+def drain(e, seqs):
+    while any(not s.finish_reason for s in seqs):
+        e.step()
+    return [s.output_ids for s in seqs]
+
+
+# ---------------------------------------------------------------- the 8-bit cache
+
+@pytest.mark.parametrize("dev", DEVICES)
+def test_chunks_steps_and_mixed_steps(dev):
+    """Prompts longer than a step's budget, arrivals while others decode, a shared prefix: the same sequences come out whether they run
+    alone or together, and logits stay near those of the unrounded cache."""
+    kw = dict(max_prefill_tokens=48, mixed_prefill_tokens=32)
+    prompts = [prompt(100, 1), prompt(17, 2), prompt(100, 1)[:64] + prompt(30, 3), prompt(5, 4)]
+    par = SamplingParams(max_tokens=12, **GREEDY)
+    e = engine(dev, kv_cache_dtype="fp8", **kw)
+    seqs = []
+    for p in prompts:
+        seqs.append(e.add_request(p, par))
+        e.step()
+        e.step()
+    together = drain(e, seqs)
+    assert all(len(o) == 12 for o in together)
+    assert e.runner.n_steps.get("mixed", 0) > 0 and e.runner.n_steps["prefill_context_tokens"] > 0
+    if dev == "cpu":  # fp32 rows: a sequence's pages do not depend on what runs beside it, only on where its prompt was cut
+        alone = engine(dev, kv_cache_dtype="fp8", prefix_caching=False, **kw)
+        for p, o in zip(prompts[1::2], together[1::2]):
+            assert drain(alone, [alone.add_request(p, par)])[0] == o
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+def test_logits_are_near_those_of_the_unrounded_cache(dev):
+    """Step after step on the same tokens: an e4m3 number is off by at most half a step, 2^-4 relative - values by that, probabilities by no more
+    where scores are of size 1 -, in each of two layers, whose sum with the residual stream the norms do not amplify: 2 * 2 * 2^-4 of the
+    logits' norm."""
+    p = prompt(60, 7)
+    got = []
+    for kind in ("auto", "fp8"):
+        e = engine(dev, kv_cache_dtype=kind, keep_logits=True, pipeline=False)
+        s = e.add_request(p, SamplingParams(max_tokens=20, **GREEDY))
+        rows = []
+        while not s.finish_reason:
+            e.step()
+            # (a replayed step's logits lie in its own buffer)
+            rows.append((e.runner.last_logits[-1] if len(s.output_ids) == 1 else e.runner.d_logits[0]).float().cpu().clone())
+            if got:
+                s.output_ids[-1] = got[0][1][len(s.output_ids) - 1]  # the same tokens on both sides
+        got.append((torch.stack(rows), list(s.output_ids)))
+    a, b = got[0][0], got[1][0]
+    assert a.shape == b.shape and float((a - b).norm() / a.norm()) <= 0.25
+    assert not torch.equal(a[5:], b[5:])
+
+
+def test_the_cache_takes_half_the_memory():
+    a, b = engine("cpu", num_blocks=None, kv_cache_gb=0.01, dtype="bfloat16"), engine("cpu", num_blocks=None, kv_cache_gb=0.01, dtype="bfloat16", kv_cache_dtype="fp8")
+    assert b.runner.num_blocks > 1.95 * a.runner.num_blocks
+    assert b.runner.memory_report()["kv_cache_bytes"] <= 0.01 * (1 << 30)
+
+
+def test_gpt2_heads_run_over_the_8_bit_cache():
+    e = engine("cpu", model="gpt2-tiny", max_model_len=128, num_blocks=32, kv_cache_dtype="fp8", max_prefill_tokens=16)
+    assert len(drain(e, [e.add_request(prompt(40, 3), SamplingParams(max_tokens=3, **GREEDY))])[0]) == 3
+
+
+def test_refused_configurations():
+    with pytest.raises(ValueError, match="kv_cache_dtype"):
+        engine("cpu", kv_cache_dtype="int4")
+    with pytest.raises(ValueError, match="head size"):
+        engine("cpu", model="llama-tiny", kv_cache_dtype="fp8", model_overrides=dict(head_dim=32, n_heads=4, n_kv_heads=2))
+
+
+# ---------------------------------------------------------------- controls
+
+def oracle(e, ids, n, p):
+    """Greedy under the controls, from whole forwards."""
+    out = []
+    for _ in range(n):
+        x = _logits(e, ids + out).double()
+        seen = sorted(set(ids + out))
+        t = x[seen]
+        x[seen] = torch.where(t > 0, t / p.repetition_penalty, t * p.repetition_penalty)
+        for v in set(out):
+            x[v] -= p.frequency_penalty * out.count(v) + p.presence_penalty
+        for v, a in (p.logit_bias or {}).items():
+            x[v] += a
+        if p.allowed_token_ids is not None:
+            keep = torch.full_like(x, float("-inf"))
+            keep[list(p.allowed_token_ids)] = 0
+            x = x + keep
+        out.append(int(x.argmax()))
+    return out
+
+
+PARAMS = [dict(repetition_penalty=1.7), dict(presence_penalty=1.5, frequency_penalty=0.8), dict(logit_bias={11: 4.0, 12: -100.0, 13: 3.5}),
+          dict(allowed_token_ids=(5, 9, 77, 200), repetition_penalty=1.3), dict(frequency_penalty=-0.5), {}]
+
+
+@pytest.mark.parametrize("pipeline", [True, False])
+def test_controlled_answers_are_the_definitions(pipeline):
+    """Together, on four sequence slots, with chunks, mixed and pipelined steps: each answer is what whole forwards and the definition give."""
+    e = engine("cpu", logit_controls=True, pipeline=pipeline, max_prefill_tokens=24, mixed_prefill_tokens=16)
+    prompts = [prompt(30 + 7 * i, 20 + i) for i in range(len(PARAMS))]
+    pars = [SamplingParams(max_tokens=8, **GREEDY, **k) for k in PARAMS]
+    seqs = [e.add_request(p, q) for p, q in zip(prompts, pars)]
+    got = drain(e, seqs)
+    for ids, p, o in zip(prompts, pars, got):
+        assert o == oracle(e, ids, 8, p)
+
+
+def _logits(e, ids):
+    """The last row's logits of a whole forward without a cache."""
+    from k8s_llm_monitor_amd.models.llama import AttnMeta
+    t = torch.tensor(ids, dtype=torch.int32)
+    meta = AttnMeta(is_prefill=True, positions=torch.arange(len(ids), dtype=torch.int32), slot_mapping=torch.full((len(ids),), -1, dtype=torch.int32),
+                    cu_seqlens=torch.tensor([0, len(ids)], dtype=torch.int32), logits_idx=torch.tensor([len(ids) - 1]))
+    return e.model.forward(t, meta, None)[0].float()
+
+
+def test_more_requests_than_slots_and_preemption():
+    """Twelve controlled requests on three sequence slots and few pages: control slots come back, preempted sequences get new ones."""
+    e = engine("cpu", logit_controls=True, max_num_seqs=3, num_blocks=14, max_model_len=96, prefix_caching=False)
+    pars = [SamplingParams(max_tokens=30, **GREEDY, **PARAMS[i % len(PARAMS)]) for i in range(12)]
+    prompts = [prompt(40 + i, 50 + i) for i in range(12)]
+    got = drain(e, [e.add_request(p, q) for p, q in zip(prompts, pars)])
+    assert e.counters["preemptions"] > 0
+    for i in (0, 3, 4, 9):
+        assert got[i] == oracle(e, prompts[i], 30, pars[i])
+
+
+@pytest.mark.gpu
+def test_controlled_answers_on_the_gpu():
+    """Captured, pipelined steps: allowed tokens only, no token twice under a presence penalty that outweighs every logit, a bias that
+    decides, beside a row without controls that answers as in an engine without them."""
+    plain = engine("cuda")
+    e = engine("cuda", logit_controls=True)
+    allowed = tuple(range(40, 60))
+    ks = [dict(allowed_token_ids=allowed, presence_penalty=1e4), {}, dict(logit_bias={123: 1e4}), dict(presence_penalty=1e4)]
+    prompts = [prompt(50, 80 + i) for i in range(4)]
+    got = drain(e, [e.add_request(p, SamplingParams(max_tokens=16, **GREEDY, **k)) for p, k in zip(prompts, ks)])
+    assert set(got[0]) <= set(allowed) and len(set(got[0])) == 16
+    assert got[1] == drain(plain, [plain.add_request(prompts[1], SamplingParams(max_tokens=16, **GREEDY))])[0]
+    assert got[2] == [123] * 16 and len(set(got[3])) == 16
+
+
+@pytest.mark.gpu
+def test_both_together_on_the_gpu():
+    e = engine("cuda", logit_controls=True, kv_cache_dtype="fp8", max_prefill_tokens=64)
+    seqs = [e.add_request(prompt(90, 90 + i), SamplingParams(max_tokens=24, temperature=0.8, top_k=20, ignore_eos=True, allowed_token_ids=tuple(range(i, 250, 3)),
+                                                             repetition_penalty=1.1)) for i in range(3)]
+    for i, o in enumerate(drain(e, seqs)):
+        assert len(o) == 24 and all(t % 3 == i for t in o)
+
+
+def test_refused_requests():
+    e = engine("cpu")
+    with pytest.raises(ValueError, match="logit_controls"):
+        e.add_request([5, 6], SamplingParams(presence_penalty=1.0))
+    e = engine("cpu", logit_controls=True, max_logit_bias=2)
+    V = e.model_cfg.vocab_size
+    for bad in (dict(repetition_penalty=0.0), dict(logit_bias={V: 1.0}), dict(logit_bias={1: 1.0, 2: 1.0, 3: 1.0}), dict(allowed_token_ids=()),
+                dict(allowed_token_ids=(-1,)), dict(frequency_penalty=float("nan"))):
+        with pytest.raises(ValueError):
+            e.add_request([5, 6], SamplingParams(**bad))
+    assert not e.has_work()
+    svc = EngineService(e)
+    try:
+        with pytest.raises(ValueError):
+            svc.submit([5, 6], SamplingParams(logit_bias={V: 1.0})).result(timeout=30)
+        assert svc.submit([5, 6], SamplingParams(max_tokens=2, **GREEDY, logit_bias={7: 1e4})).result(timeout=60)[1].output_ids == [7, 7]
+    finally:
+        svc.close()
+
+
+def test_chat_requests_have_them():
+    """POST /v1/chat/completions: presence_penalty, frequency_penalty, logit_bias reach a backend that takes them; 400 for what it refuses."""
+    from k8s_llm_monitor_amd.monitor.server import MonitorApp, _chat_controls
+    assert _chat_controls({"presence_penalty": 1, "logit_bias": {"7": -2}}) == {"presence_penalty": 1.0, "logit_bias": {7: -2.0}}
+    for bad in ({"presence_penalty": "x"}, {"logit_bias": {"a": 1}}, {"logit_bias": [1]}, {"frequency_penalty": True}):
+        with pytest.raises(Exception) as err:
+            _chat_controls(bad)
+        assert err.value.code == 400
+
+    class Backend:
+        takes_controls = True
+
+        def generate(self, prompt, max_tokens=None, temperature=None, top_p=None, controls=None):
+            if controls and 9 in controls.get("logit_bias", {}):
+                raise ValueError("token 9")
+            return {"text": json.dumps(controls), "model": "m"}
+
+    class Analysis:
+        backend = Backend()
+
+        def fit_chat(self, parts, mt):
+            return "\n".join(parts)
+
+    app = MonitorApp.__new__(MonitorApp)
+    app.analysis = Analysis()
+    app._bounded = lambda fn: fn()
+    ask = lambda **k: app.chat_completions("POST", json.dumps({"messages": [{"role": "user", "content": "hi"}], **k}).encode(), {})  # noqa: E731
+    text = lambda r: json.loads(r.body)["choices"][0]["message"]["content"]  # noqa: E731
+    assert json.loads(text(ask(frequency_penalty=0.5))) == {"frequency_penalty": 0.5}
+    assert text(ask()) == "null"
+    with pytest.raises(Exception) as err:
+        ask(logit_bias={"9": 1})
+    assert err.value.code == 400
+    Backend.takes_controls = False
+    assert text(ask(frequency_penalty=0.5)) == "null"
