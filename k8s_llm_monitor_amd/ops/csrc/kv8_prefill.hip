@@ -58,17 +58,19 @@ __global__ __launch_bounds__(512, 2) void kv8_prefill_kernel(const Kv8Prefill a)
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int r32 = lane & 31, hh = lane >> 5;
-  const int cst = max(0, min(a.ctx[seq], a.table_width * kPage - L));  // keys never pass the table
+  const int cst = __builtin_amdgcn_readfirstlane(max(0, min(a.ctx[seq], a.table_width * kPage - L)));  // keys never pass the table
   const int LK = cst + L, last_page = min((LK - 1) >> 4, a.table_width - 1);
   const int f = f0 + 32 * wave + r32;
   const bool mine = f < pairs;
   const int row = qs + (mine ? f / G : 0), hq = kvh * G + (mine ? f % G : 0);
-  const int wave_first = cst + qs + (f0 + 32 * wave) / G;  // position of the wave's first row
+  // (divisions are done in vector registers: what branches hang on goes back to scalar ones)
+  const int wave_first = __builtin_amdgcn_readfirstlane(cst + qs + (f0 + 32 * wave) / G);  // position of the wave's first row
   const bool busy = f0 + 32 * wave < pairs;
   const int wave_last = cst + qs + (min(pairs, f0 + 32 * wave + 32) - 1) / G;
   const int tiles = (cst + qs + (min(pairs, f0 + 256) - 1) / G) / kTile + 1;
-  const int per = (tiles + a.S - 1) / a.S, tb = blockIdx.z * per, te = min(tiles, tb + per);
-  const int nt = busy ? min(te, wave_last / kTile + 1) : 0;  // the wave's tiles end here
+  const int per = (tiles + a.S - 1) / a.S;
+  const int tb = __builtin_amdgcn_readfirstlane(blockIdx.z * per), te = __builtin_amdgcn_readfirstlane(min(tiles, tb + per));
+  const int nt = __builtin_amdgcn_readfirstlane(busy ? min(te, wave_last / kTile + 1) : 0);  // the wave's tiles end here
 
   bf16x8 qf[KS];
   {
@@ -81,7 +83,7 @@ __global__ __launch_bounds__(512, 2) void kv8_prefill_kernel(const Kv8Prefill a)
   // ---- staging: thread = (page of the tile, 16 bytes of it); D = 128: all threads K and V, D = 64: the lower half K, the upper V
   constexpr bool BOTH = D == 128;
   const int piece = BOTH ? tid : tid & 255;
-  const bool has_k = BOTH || tid < 256, has_v = BOTH || tid >= 256;
+  const bool has_k = BOTH || wave < 4, has_v = BOTH || wave >= 4;  // uniform in a wave
   const int pg = piece / (D);  // page of the tile: D pieces of 16 bytes a page
   const int in = piece & (D - 1);
   // K piece: [run kg][half of the run's dims][token]: the lanes of a store hold one token each side by side
@@ -102,23 +104,19 @@ __global__ __launch_bounds__(512, 2) void kv8_prefill_kernel(const Kv8Prefill a)
     r.ks = a.scales[tile * 2];
     r.vs = a.scales[tile * 2 + 1];
   };
-  auto stage = [&](Raw& r, int t) {
-    bf16_t *kt = s_k[t & 1], *vt = s_v[t & 1];
-    if (has_k) {
-      bf16_t* p = kt + (2 * kpart * kTile + pg * kPage + ktok) * 8;
-      *reinterpret_cast<bf16x8*>(p) = kv8_values(r.k[0], r.k[1], r.ks);
-      *reinterpret_cast<bf16x8*>(p + kTile * 8) = kv8_values(r.k[2], r.k[3], r.ks);
+  // Tile t's codes before they are converted: those behind the sequence's end, where a page holds anything, and NaN ones become zero
+  auto settle = [&](Raw& r, int t) {
+    if (!has_v) return;
+    const int left = LK - (t * kTile + pg * kPage);
+    if (__builtin_amdgcn_readfirstlane(left) < kPage) {
+#pragma unroll
+      for (int w = 0; w < 4; ++w) r.v[w] &= kv8_below(left, w);
+      if (left <= 0) r.vs = 1.f;
     }
-    if (has_v) {
-      const int left = LK - (t * kTile + pg * kPage);
-      if (left < kPage) {  // behind the sequence's end a page holds anything
+    uint32_t bad[4], any = 0;  // the high bit of each NaN code (0x7f, 0xff)
 #pragma unroll
-        for (int w = 0; w < 4; ++w) r.v[w] &= kv8_below(left, w);
-        if (left <= 0) r.vs = 1.f;
-      }
-      uint32_t bad[4], any = 0;  // the high bit of each NaN code (0x7f, 0xff)
-#pragma unroll
-      for (int w = 0; w < 4; ++w) any |= bad[w] = ((r.v[w] & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u;
+    for (int w = 0; w < 4; ++w) any |= bad[w] = ((r.v[w] & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u;
+    if (__builtin_amdgcn_ballot_w64(any != 0)) {
       if (any) {
         int first = 0;
 #pragma unroll
@@ -128,8 +126,17 @@ __global__ __launch_bounds__(512, 2) void kv8_prefill_kernel(const Kv8Prefill a)
 #pragma unroll
         for (int w = 0; w < 4; ++w) r.v[w] &= ~((bad[w] >> 7) * 0xffu);
       }
+    }
+  };
+  auto stage = [&](const Raw& r, int t) {
+    if (has_k) {
+      bf16_t* p = s_k[t & 1] + (2 * kpart * kTile + pg * kPage + ktok) * 8;
+      *reinterpret_cast<bf16x8*>(p) = kv8_values(r.k[0], r.k[1], r.ks);
+      *reinterpret_cast<bf16x8*>(p + kTile * 8) = kv8_values(r.k[2], r.k[3], r.ks);
+    }
+    if (has_v) {
       // the 8 tokens of the accumulator's half hh: 0-3, 8-11 and 4-7, 12-15; the two chunks of a dim change places by its bit 3
-      bf16_t* p = vt + (pg * D + in) * 16;
+      bf16_t* p = s_v[t & 1] + (pg * D + in) * 16;
       const int x = ((in >> 3) & 1) * 8;
       *reinterpret_cast<bf16x8*>(p + x) = kv8_values(r.v[0], r.v[2], r.vs);
       *reinterpret_cast<bf16x8*>(p + (8 - x)) = kv8_values(r.v[1], r.v[3], r.vs);
@@ -143,7 +150,8 @@ __global__ __launch_bounds__(512, 2) void kv8_prefill_kernel(const Kv8Prefill a)
     for (int r = 0; r < 16; ++r) o[d][r] = 0.f;
   float m = -1e30f, l = 0.f;
 
-  auto scores = [&](int t, f32x16 (&s)[2]) {
+  // S^T of tile t, tile t + 1's conversions and LDS stores between its products: they are this wave's only other work then
+  auto scores = [&](int t, f32x16 (&s)[2], Raw& r) {
     const bf16_t* kt = s_k[t & 1];
     bf16x8 kf[KS][2];
 #pragma unroll
@@ -155,10 +163,21 @@ __global__ __launch_bounds__(512, 2) void kv8_prefill_kernel(const Kv8Prefill a)
 #pragma unroll
       for (int r = 0; r < 16; ++r) s[i][r] = 0.f;
     __builtin_amdgcn_sched_barrier(0);
+    asm volatile("" : "+v"(r.k), "+v"(r.v));  // (the conversions stay here and do not move ahead of the branch)
+    stage(r, t + 1);
 #pragma unroll
     for (int ks = 0; ks < KS; ++ks)
 #pragma unroll
       for (int i = 0; i < 2; ++i) s[i] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf[ks][i], qf[ks], s[i], 0, 0, 0);
+    if constexpr (BOTH) {
+#pragma unroll
+      for (int n = 0; n < 2 * KS; ++n) {
+        __builtin_amdgcn_sched_group_barrier(0x8, 1, 0);    // a product
+        __builtin_amdgcn_sched_group_barrier(0x2, 2, 0);    // vector instructions
+        __builtin_amdgcn_sched_group_barrier(0x200, 1, 0);  // an LDS store
+      }
+    }
+    __builtin_amdgcn_sched_barrier(0);
     if (t * kTile + kTile - 1 > wave_first) {  // keys past this lane's row (uniform branch)
       const int lim = cst + row - t * kTile - 4 * hh;
 #pragma unroll
@@ -218,23 +237,28 @@ __global__ __launch_bounds__(512, 2) void kv8_prefill_kernel(const Kv8Prefill a)
   };
 
   if (tb < te) {
-    Raw r;  // the tile behind the one that is multiplied
+    Raw r;  // the tile behind the one that is multiplied (behind the last one: its last page again)
     fetch(r, page_of(tb));
     int next = page_of(tb + 1);
     __syncthreads();  // s_nan
+    settle(r, tb);
     stage(r, tb);
     fetch(r, next);
     next = page_of(tb + 2);
     for (int t = tb; t < te; ++t) {
       __syncthreads();
-      f32x16 s[2];
-      if (t < nt) scores(t, s);
-      if (t + 1 < te) {
+      settle(r, t + 1);
+      if (t < nt) {
+        f32x16 s[2];
+        scores(t, s, r);
+        fetch(r, next);
+        next = page_of(t + 3);
+        products(t, s);
+      } else {
         stage(r, t + 1);
         fetch(r, next);
         next = page_of(t + 3);
       }
-      if (t < nt) products(t, s);
     }
     __syncthreads();  // s_nan
   }
