@@ -40,12 +40,14 @@ struct Kv8Prefill {
 };
 
 constexpr int kTile = 64;
+typedef int i32x8 __attribute__((ext_vector_type(8)));
 
 template <int D>
 __global__ __launch_bounds__(512, 2) void kv8_prefill_kernel(const Kv8Prefill a) {
-  constexpr int KS = D / 16, DT = D / 32, KD = D / 4, CH = D / 8;
+  constexpr int KS = D / 64, DT = D / 32, KD = D / 4;
   constexpr int kHalf = kTile * D;  // elements of a K (or V) tile
-  __shared__ __attribute__((aligned(16))) bf16_t s_k[2][kHalf];  // [D / 8][64 keys][8]
+  __shared__ __attribute__((aligned(16))) uint8_t s_k[2][kHalf];  // [4 pages][4 runs][16 tokens][D / 4], codes
+  __shared__ uint32_t s_kscale[2][4];                             // the pages' scales as e8m0
   __shared__ __attribute__((aligned(16))) bf16_t s_v[2][kHalf];  // [4 pages][D][2 chunks of 8 tokens]
   __shared__ int s_nan[D];  // first token whose V code is NaN
 
@@ -72,11 +74,29 @@ __global__ __launch_bounds__(512, 2) void kv8_prefill_kernel(const Kv8Prefill a)
   const int tb = __builtin_amdgcn_readfirstlane(blockIdx.z * per), te = __builtin_amdgcn_readfirstlane(min(tiles, tb + per));
   const int nt = __builtin_amdgcn_readfirstlane(busy ? min(te, wave_last / kTile + 1) : 0);  // the wave's tiles end here
 
-  bf16x8 qf[KS];
+  // q as the sum of two e4m3 numbers, the second a sixteenth as large: a code's 4 bits and the 4 of what it leaves off are bf16's 8, so this
+  // is q itself but for numbers below 2^-15 of the row's largest, which are off by 2^-22 of it
+  i32x8 q_hi[KS], q_lo[KS];
+  uint32_t qs_hi[KS];
   {
-    const bf16_t* qp = a.qkv + (long)(s0 + row) * a.qkv_stride + hq * D + 8 * hh;
+    const bf16_t* qp = a.qkv + (long)(s0 + row) * a.qkv_stride + hq * D + 32 * hh;
 #pragma unroll
-    for (int ks = 0; ks < KS; ++ks) qf[ks] = *reinterpret_cast<const bf16x8*>(qp + 16 * ks);
+    for (int ks = 0; ks < KS; ++ks) {
+      float x[32], amax = 0.f;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) unpack8(*reinterpret_cast<const uint4*>(qp + 64 * ks + 8 * j), x + 8 * j);
+#pragma unroll
+      for (int j = 0; j < 32; ++j) amax = fmaxf(amax, kv8_finite(x[j]));
+      const float sc = kv8_scale(xor32_max_f(amax)), inv = kv8_inverse(sc);
+      qs_hi[ks] = __float_as_uint(sc) >> 23;
+#pragma unroll
+      for (int w = 0; w < 8; ++w) {
+        const uint32_t hi = kv8_codes(x[4 * w], x[4 * w + 1], x[4 * w + 2], x[4 * w + 3], inv);
+        const f32x2 u = __builtin_amdgcn_cvt_pk_f32_fp8(hi, false), v = __builtin_amdgcn_cvt_pk_f32_fp8(hi, true);
+        q_hi[ks][w] = (int)hi;
+        q_lo[ks][w] = (int)kv8_codes(x[4 * w] - u[0] * sc, x[4 * w + 1] - u[1] * sc, x[4 * w + 2] - v[0] * sc, x[4 * w + 3] - v[1] * sc, 16.f * inv);
+      }
+    }
   }
   for (int i = tid; i < D; i += 512) s_nan[i] = 0x7fffffff;
 
@@ -86,7 +106,8 @@ __global__ __launch_bounds__(512, 2) void kv8_prefill_kernel(const Kv8Prefill a)
   const bool has_k = BOTH || wave < 4, has_v = BOTH || wave >= 4;  // uniform in a wave
   const int pg = piece / (D);  // page of the tile: D pieces of 16 bytes a page
   const int in = piece & (D - 1);
-  // K piece: [run kg][half of the run's dims][token]: the lanes of a store hold one token each side by side
+  // K piece: [run][half of its dims, D = 128][token]; the halves of a token's run change places from its eighth token on, so that sixteen lanes'
+  // reads of one half meet all banks
   const int ktok = in & 15, kpart = in >> 4;  // 16-dim parts 0 .. D / 16 - 1: dims 16 kpart ..
   const int k_src = ((kpart * 16) / KD * kPage + ktok) * KD + (kpart * 16) % KD;
   int zero;  // in a vector register: page numbers and scales are loaded as vectors are, not by scalar loads, whose counter is LDS's
@@ -130,9 +151,8 @@ __global__ __launch_bounds__(512, 2) void kv8_prefill_kernel(const Kv8Prefill a)
   };
   auto stage = [&](const Raw& r, int t) {
     if (has_k) {
-      bf16_t* p = s_k[t & 1] + (2 * kpart * kTile + pg * kPage + ktok) * 8;
-      *reinterpret_cast<bf16x8*>(p) = kv8_values(r.k[0], r.k[1], r.ks);
-      *reinterpret_cast<bf16x8*>(p + kTile * 8) = kv8_values(r.k[2], r.k[3], r.ks);
+      *reinterpret_cast<u32x4*>(s_k[t & 1] + pg * (kPage * D) + (D == 128 ? k_src ^ ((ktok & 8) << 1) : k_src)) = r.k;
+      if (in == 0) s_kscale[t & 1][pg] = __float_as_uint(r.ks) >> 23;
     }
     if (has_v) {
       // the 8 tokens of the accumulator's half hh: 0-3, 8-11 and 4-7, 12-15; the two chunks of a dim change places by its bit 3
@@ -152,12 +172,31 @@ __global__ __launch_bounds__(512, 2) void kv8_prefill_kernel(const Kv8Prefill a)
 
   // S^T of tile t, tile t + 1's conversions and LDS stores between its products: they are this wave's only other work then
   auto scores = [&](int t, f32x16 (&s)[2], Raw& r) {
-    const bf16_t* kt = s_k[t & 1];
-    bf16x8 kf[KS][2];
+    // key 32 i + r32: page 2 i + (r32 >> 4), token r32 & 15; dims 64 ks + 32 hh ..: runs of D / 4
+    const uint8_t* kt = s_k[t & 1];
+    i32x8 kf[KS][2];
+    uint32_t sc[2];
 #pragma unroll
-    for (int ks = 0; ks < KS; ++ks)
+    for (int i = 0; i < 2; ++i) {
+      const int pg = 2 * i + (r32 >> 4), tok = r32 & 15;
+      sc[i] = s_kscale[t & 1][pg];
 #pragma unroll
-      for (int i = 0; i < 2; ++i) kf[ks][i] = *reinterpret_cast<const bf16x8*>(kt + ((2 * ks + hh) * kTile + 32 * i + r32) * 8);
+      for (int ks = 0; ks < KS; ++ks) {
+        const uint8_t* p = kt + pg * (kPage * D);
+        u32x4 lo, hi;
+        if constexpr (D == 128) {
+          p += ((2 * ks + hh) * kPage + tok) * KD;
+          const int x = (tok & 8) << 1;
+          lo = *reinterpret_cast<const u32x4*>(p + x);
+          hi = *reinterpret_cast<const u32x4*>(p + (16 - x));
+        } else {
+          p += (2 * hh * kPage + tok) * KD;
+          lo = *reinterpret_cast<const u32x4*>(p);
+          hi = *reinterpret_cast<const u32x4*>(p + kPage * KD);
+        }
+        kf[ks][i] = i32x8{(int)lo[0], (int)lo[1], (int)lo[2], (int)lo[3], (int)hi[0], (int)hi[1], (int)hi[2], (int)hi[3]};
+      }
+    }
 #pragma unroll
     for (int i = 0; i < 2; ++i)
 #pragma unroll
@@ -168,10 +207,14 @@ __global__ __launch_bounds__(512, 2) void kv8_prefill_kernel(const Kv8Prefill a)
 #pragma unroll
     for (int ks = 0; ks < KS; ++ks)
 #pragma unroll
-      for (int i = 0; i < 2; ++i) s[i] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf[ks][i], qf[ks], s[i], 0, 0, 0);
+      for (int part = 0; part < 2; ++part)
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+          s[i] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(kf[ks][i], part ? q_lo[ks] : q_hi[ks], s[i], 0, 0, 0, (int)sc[i], 0,
+                                                                 (int)(part ? qs_hi[ks] - 4 : qs_hi[ks]));
     if constexpr (BOTH) {
 #pragma unroll
-      for (int n = 0; n < 2 * KS; ++n) {
+      for (int n = 0; n < 4 * KS; ++n) {
         __builtin_amdgcn_sched_group_barrier(0x8, 1, 0);    // a product
         __builtin_amdgcn_sched_group_barrier(0x2, 2, 0);    // vector instructions
         __builtin_amdgcn_sched_group_barrier(0x200, 1, 0);  // an LDS store
