@@ -14,7 +14,7 @@ int k8sllm_kv8_decode(void* out, long out_stride, float* part_o, float* part_ml,
                       int pages, const int* table, long table_stride, int table_width, const int* lens, int B, int Hq, int Hkv, int D, int S,
                       float scale, int* ctr, const float* slabs, int nslabs, const int* positions, const float* cos_sin, int max_pos,
                       const int* slots, hipStream_t s);
-int k8sllm_kv8_prefill_splits(int n_qblocks, int Hq, int Hkv, int table_width);
+int k8sllm_kv8_prefill_splits(int n_qblocks, int rows, int Hq, int Hkv, int table_width);
 int k8sllm_kv8_prefill(void* out, long out_stride, const void* qkv, long qkv_stride, const int* cu, const int* ctx, const int* qb_seq,
                        const int* qb_start, int n_qblocks, int seqs, int rows, int Hq, int Hkv, int D, float scale, const void* k, const void* v,
                        const float* scales, int pages, const int* table, long table_stride, int table_width, int S, float* part_o, float* part_ml,
@@ -217,7 +217,7 @@ void kv8_prefill(Tensor out, Tensor qkv, Tensor cu, Tensor ctx, Tensor qb_seq, T
                   (uintptr_t)out.data_ptr() % 8 == 0, c.what, ": out must be [T, Hq * D], from 8 bytes on");
   TORCH_CHECK(nq * ((128 * (Hq / Hkv) + 255) / 256) <= 65535 && T < (1LL << 30), c.what, ": too many q-blocks");
   if (T == 0 || nq == 0) return;
-  const int S = k8sllm_kv8_prefill_splits((int)nq, h.Hq, h.Hkv, t.width);
+  const int S = k8sllm_kv8_prefill_splits((int)nq, (int)T, h.Hq, h.Hkv, t.width);
   Tensor po, pml;
   if (S > 1) {  // the allocator's, on this stream: a later call on it may take them again when this one is done
     po = torch::empty({S, T, Hq, D}, qkv.options().dtype(torch::kFloat32));

@@ -2,21 +2,32 @@
 // - what came before and the chunk itself - are read from the pages, so that a prompt's answer does not depend on where it was cut.
 //
 // A workgroup takes one kv head and 256 (query row, head of the group) pairs, pair f = row * G + g, 32 to a wave: any group size fills
-// the v_mfma_f32_32x32x16_bf16 columns, and the heads of a row share every K / V tile.  Products are in the swapped orientation
+// the 32-column MFMAs, and the heads of a row share every K / V tile.  Products are in the swapped orientation
 //   S^T[key][pair] = K Q^T,   O^T[dim][pair] += V^T P^T
 // so running maximum, sum and the accumulator's rescale are lane-local but for one exchange of the wave's halves, and the score
 // accumulator, rounded to bf16, is the second product's operand in place.
 //
-// Tiles of 64 keys (4 pages).  A thread loads 16 bytes of K codes and 16 of V codes a tile, one tile ahead, and turns them to bf16 on
-// their way into LDS (8 conversions of two codes each, with the page's scale in them: exact); done by each wave for itself behind LDS it would
-// be eight times that.  Two bf16 tiles of 2 * 64 * D * 2 bytes in LDS, one barrier a tile: at tile t's barrier all waves are done
-// with tile t - 1, whose half takes tile t + 1 under tile t's products.
+// Scores are v_mfma_scale_f32_32x32x64_f8f6f4 on the codes as they lie, with the page's scale as the operand's: K is staged without a
+// conversion and read from LDS at half the bytes.  q is the sum of two e4m3 numbers (see there), so nothing of bf16's precision is lost; two
+// products at twice the rate cost what one in bf16 does.  (In bf16, K converted on its way: 908 us for the last figure below, 825 so.)
+// Probabilities as two e4m3 numbers would spare V's conversion but cost more in vector instructions than it does.
+//
+// Tiles of 64 keys (4 pages).  A thread loads 16 bytes of K codes and 16 of V codes a tile, a tile ahead of their way into LDS, where V
+// becomes bf16 (8 conversions of two codes each, with the page's scale in them: exact); done by each wave for itself behind LDS it would be eight times
+// that.  Staging goes between the wave's score products.  Four buffers of 24 KB (D = 128) and a barrier every other tile: waves drift apart by
+// up to two tiles, and the second half of a tile - exponentials and the second product, both units at work - has priority over another
+// wave's first, so that the two waves of a SIMD are in different halves more often than not (a barrier a tile, or no priority: 828 and
+// 835 us for 807).  Bound by MFMAs, LDS reads and exponentials in about equal parts: a tile's 32 and 64 KB of the eight waves' reads
+// and 2 x 1000 cycles of vector instructions take 2000 cycles each.
 //
 // A V code that is NaN counts for rows that see its token and no others, though all rows of a tile multiply it (0 * NaN): the tile is
 // staged with zero in its place, and the first such token of each dim is kept and put on the rows behind it at the end.
 //
 // Few rows (a short question behind a long conversation) leave most of the chip idle: the keys are then split S ways and fp32 partials
 // joined by a second launch.
+//
+// Measured: 4096 rows behind 12 k tokens, 32 heads over 8: 807 us, 1.19 PFLOP/s (a large bf16 library product: 1.36); 10 x 1124 rows behind 512: 222 us,
+// 0.80; 45 rows behind 4 k tokens: 23 us.
 #include <algorithm>
 
 #include "kv8.h"
@@ -46,9 +57,9 @@ template <int D>
 __global__ __launch_bounds__(512, 2) void kv8_prefill_kernel(const Kv8Prefill a) {
   constexpr int KS = D / 64, DT = D / 32, KD = D / 4;
   constexpr int kHalf = kTile * D;  // elements of a K (or V) tile
-  __shared__ __attribute__((aligned(16))) uint8_t s_k[2][kHalf];  // [4 pages][4 runs][16 tokens][D / 4], codes
-  __shared__ uint32_t s_kscale[2][4];                             // the pages' scales as e8m0
-  __shared__ __attribute__((aligned(16))) bf16_t s_v[2][kHalf];  // [4 pages][D][2 chunks of 8 tokens]
+  __shared__ __attribute__((aligned(16))) uint8_t s_k[4][kHalf];  // [4 pages][4 runs][16 tokens][D / 4], codes
+  __shared__ uint32_t s_kscale[4][4];                             // the pages' scales as e8m0
+  __shared__ __attribute__((aligned(16))) bf16_t s_v[4][kHalf];  // [4 pages][D][2 chunks of 8 tokens]
   __shared__ int s_nan[D];  // first token whose V code is NaN
 
   const int kvh = blockIdx.x, qb = blockIdx.y / a.Z, G = a.G;
@@ -74,30 +85,6 @@ __global__ __launch_bounds__(512, 2) void kv8_prefill_kernel(const Kv8Prefill a)
   const int tb = __builtin_amdgcn_readfirstlane(blockIdx.z * per), te = __builtin_amdgcn_readfirstlane(min(tiles, tb + per));
   const int nt = __builtin_amdgcn_readfirstlane(busy ? min(te, wave_last / kTile + 1) : 0);  // the wave's tiles end here
 
-  // q as the sum of two e4m3 numbers, the second a sixteenth as large: a code's 4 bits and the 4 of what it leaves off are bf16's 8, so this
-  // is q itself but for numbers below 2^-15 of the row's largest, which are off by 2^-22 of it
-  i32x8 q_hi[KS], q_lo[KS];
-  uint32_t qs_hi[KS];
-  {
-    const bf16_t* qp = a.qkv + (long)(s0 + row) * a.qkv_stride + hq * D + 32 * hh;
-#pragma unroll
-    for (int ks = 0; ks < KS; ++ks) {
-      float x[32], amax = 0.f;
-#pragma unroll
-      for (int j = 0; j < 4; ++j) unpack8(*reinterpret_cast<const uint4*>(qp + 64 * ks + 8 * j), x + 8 * j);
-#pragma unroll
-      for (int j = 0; j < 32; ++j) amax = fmaxf(amax, kv8_finite(x[j]));
-      const float sc = kv8_scale(xor32_max_f(amax)), inv = kv8_inverse(sc);
-      qs_hi[ks] = __float_as_uint(sc) >> 23;
-#pragma unroll
-      for (int w = 0; w < 8; ++w) {
-        const uint32_t hi = kv8_codes(x[4 * w], x[4 * w + 1], x[4 * w + 2], x[4 * w + 3], inv);
-        const f32x2 u = __builtin_amdgcn_cvt_pk_f32_fp8(hi, false), v = __builtin_amdgcn_cvt_pk_f32_fp8(hi, true);
-        q_hi[ks][w] = (int)hi;
-        q_lo[ks][w] = (int)kv8_codes(x[4 * w] - u[0] * sc, x[4 * w + 1] - u[1] * sc, x[4 * w + 2] - v[0] * sc, x[4 * w + 3] - v[1] * sc, 16.f * inv);
-      }
-    }
-  }
   for (int i = tid; i < D; i += 512) s_nan[i] = 0x7fffffff;
 
   // ---- staging: thread = (page of the tile, 16 bytes of it); D = 128: all threads K and V, D = 64: the lower half K, the upper V
@@ -151,18 +138,60 @@ __global__ __launch_bounds__(512, 2) void kv8_prefill_kernel(const Kv8Prefill a)
   };
   auto stage = [&](const Raw& r, int t) {
     if (has_k) {
-      *reinterpret_cast<u32x4*>(s_k[t & 1] + pg * (kPage * D) + (D == 128 ? k_src ^ ((ktok & 8) << 1) : k_src)) = r.k;
-      if (in == 0) s_kscale[t & 1][pg] = __float_as_uint(r.ks) >> 23;
+      *reinterpret_cast<u32x4*>(s_k[t & 3] + pg * (kPage * D) + (D == 128 ? k_src ^ ((ktok & 8) << 1) : k_src)) = r.k;
+      if (in == 0) s_kscale[t & 3][pg] = __float_as_uint(r.ks) >> 23;
     }
     if (has_v) {
       // the 8 tokens of the accumulator's half hh: 0-3, 8-11 and 4-7, 12-15; the two chunks of a dim change places by its bit 3
-      bf16_t* p = s_v[t & 1] + (pg * D + in) * 16;
+      bf16_t* p = s_v[t & 3] + (pg * D + in) * 16;
       const int x = ((in >> 3) & 1) * 8;
       *reinterpret_cast<bf16x8*>(p + x) = kv8_values(r.v[0], r.v[2], r.vs);
       *reinterpret_cast<bf16x8*>(p + (8 - x)) = kv8_values(r.v[1], r.v[3], r.vs);
     }
   };
 
+  // the first two tiles are on their way while q is prepared
+  Raw r, r1;
+  int next;
+  {
+    const int p0 = page_of(tb), p1 = page_of(tb + 1);
+    next = page_of(tb + 2);
+    fetch(r, p0);
+    fetch(r1, p1);
+  }
+
+  // q as the sum of two e4m3 numbers, the second a sixteenth as large: a code's 4 bits and the 4 of what it leaves off are bf16's 8, so this
+  // is q itself but for numbers below 2^-15 of the row's largest, which are off by 2^-22 of it
+  i32x8 q_hi[KS], q_lo[KS];
+  uint32_t qs_hi[KS];
+  {
+    const bf16_t* qp = a.qkv + (long)(s0 + row) * a.qkv_stride + hq * D + 32 * hh;
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) {
+      u32x4 x[4];
+      uint32_t m = 0;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        x[j] = *reinterpret_cast<const u32x4*>(qp + 64 * ks + 8 * j);
+#pragma unroll
+        for (int w = 0; w < 4; ++w) m = kv8_max_bits(m, x[j][w]);
+      }
+      // (a row with infinities or NaN, which are NaN codes, answers NaN under any scale)
+      const float amax = fminf(fmaxf(lo_bf(m), hi_bf(m)), 3.3895314e38f);
+      const float sc = kv8_scale(xor32_max_f(amax)), sc_lo = sc * 0.0625f;
+      qs_hi[ks] = __float_as_uint(sc) >> 23;
+#pragma unroll
+      for (int w = 0; w < 8; ++w) {
+        const uint32_t a0 = x[w >> 1][2 * (w & 1)], a1 = x[w >> 1][2 * (w & 1) + 1];
+        const uint32_t hi = kv8_codes_bf16(a0, a1, sc);
+        const f32x2 u = __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(hi, sc, false), v = __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(hi, sc, true);
+        s16x2 lo = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(s16x2{0, 0}, lo_bf(a0) - u[0], hi_bf(a0) - u[1], sc_lo, false);
+        lo = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(lo, lo_bf(a1) - v[0], hi_bf(a1) - v[1], sc_lo, true);
+        q_hi[ks][w] = (int)hi;
+        q_lo[ks][w] = __builtin_bit_cast(int, lo);
+      }
+    }
+  }
   f32x16 o[DT];
 #pragma unroll
   for (int d = 0; d < DT; ++d)
@@ -170,16 +199,16 @@ __global__ __launch_bounds__(512, 2) void kv8_prefill_kernel(const Kv8Prefill a)
     for (int r = 0; r < 16; ++r) o[d][r] = 0.f;
   float m = -1e30f, l = 0.f;
 
-  // S^T of tile t, tile t + 1's conversions and LDS stores between its products: they are this wave's only other work then
+  // S^T of tile t, tile t + 2's conversions and LDS stores between its products: they are this wave's only other work then
   auto scores = [&](int t, f32x16 (&s)[2], Raw& r) {
     // key 32 i + r32: page 2 i + (r32 >> 4), token r32 & 15; dims 64 ks + 32 hh ..: runs of D / 4
-    const uint8_t* kt = s_k[t & 1];
+    const uint8_t* kt = s_k[t & 3];
     i32x8 kf[KS][2];
     uint32_t sc[2];
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
       const int pg = 2 * i + (r32 >> 4), tok = r32 & 15;
-      sc[i] = s_kscale[t & 1][pg];
+      sc[i] = s_kscale[t & 3][pg];
 #pragma unroll
       for (int ks = 0; ks < KS; ++ks) {
         const uint8_t* p = kt + pg * (kPage * D);
@@ -203,7 +232,7 @@ __global__ __launch_bounds__(512, 2) void kv8_prefill_kernel(const Kv8Prefill a)
       for (int r = 0; r < 16; ++r) s[i][r] = 0.f;
     __builtin_amdgcn_sched_barrier(0);
     asm volatile("" : "+v"(r.k), "+v"(r.v));  // (the conversions stay here and do not move ahead of the branch)
-    stage(r, t + 1);
+    stage(r, t + 2);
 #pragma unroll
     for (int ks = 0; ks < KS; ++ks)
 #pragma unroll
@@ -230,7 +259,7 @@ __global__ __launch_bounds__(512, 2) void kv8_prefill_kernel(const Kv8Prefill a)
     }
   };
   auto products = [&](int t, f32x16 (&s)[2]) {
-    const bf16_t* vt = s_v[t & 1];
+    const bf16_t* vt = s_v[t & 3];
     bf16x8 vf[2][2][DT];
 #pragma unroll
     for (int i = 0; i < 2; ++i)
@@ -280,27 +309,28 @@ __global__ __launch_bounds__(512, 2) void kv8_prefill_kernel(const Kv8Prefill a)
   };
 
   if (tb < te) {
-    Raw r;  // the tile behind the one that is multiplied (behind the last one: its last page again)
-    fetch(r, page_of(tb));
-    int next = page_of(tb + 1);
     __syncthreads();  // s_nan
     settle(r, tb);
     stage(r, tb);
-    fetch(r, next);
-    next = page_of(tb + 2);
+    settle(r1, tb + 1);
+    stage(r1, tb + 1);
+    fetch(r, next);  // from here on r is the next tile to stage (behind the last one: later keys, or the last page again)
+    next = page_of(tb + 3);
     for (int t = tb; t < te; ++t) {
-      __syncthreads();
-      settle(r, t + 1);
+      if (((t - tb) & 1) == 0) __syncthreads();
+      settle(r, t + 2);
       if (t < nt) {
         f32x16 s[2];
         scores(t, s, r);
         fetch(r, next);
-        next = page_of(t + 3);
+        next = page_of(t + 4);
+        __builtin_amdgcn_s_setprio(1);
         products(t, s);
+        __builtin_amdgcn_s_setprio(0);
       } else {
-        stage(r, t + 1);
+        stage(r, t + 2);
         fetch(r, next);
-        next = page_of(t + 3);
+        next = page_of(t + 4);
       }
     }
     __syncthreads();  // s_nan
@@ -376,16 +406,17 @@ __global__ __launch_bounds__(256) void kv8_prefill_join_kernel(const Kv8Prefill 
 
 using namespace k8sllm;
 
-// How many ways the keys are split: grids of fewer than 256 workgroups take up to 32 splits of at least 4 tiles of the longest context that
-// the block tables allow.
-extern "C" int k8sllm_kv8_prefill_splits(int n_qblocks, int Hq, int Hkv, int table_width) {
-  const int Z = (128 * (Hq / Hkv) + 255) / 256;
-  const long groups = (long)n_qblocks * Z * Hkv;
-  const long room = (long)table_width * kPage / (4 * kTile);
-  long s = (256 + groups - 1) / (groups > 0 ? groups : 1);
-  if (s > room) s = room;
-  if (s > 32) s = 32;
-  return s < 1 ? 1 : (int)s;
+// Workgroups a q-block: no block has more rows than the call
+static int prefill_z(int rows, int G) { return (std::min(128, rows) * G + 255) / 256; }
+
+// How many ways the keys are split: where the rows make fewer than 256 workgroups, up to 32 splits of at least 4 tiles of the longest context
+// that the block tables allow.  (A split's partials are 512 bytes a row and head out and in: 45 rows behind 4 k tokens, 32 heads: 16 splits
+// of 5 tiles 17.5 + 4.0 us, 32 of 3 tiles 17.4 + 5.5.)
+extern "C" int k8sllm_kv8_prefill_splits(int n_qblocks, int rows, int Hq, int Hkv, int table_width) {
+  const int G = Hq / Hkv, Z = prefill_z(rows, G);
+  const long groups = std::max(1L, std::min((long)n_qblocks * Z, (long)rows * G / 256 + n_qblocks) * Hkv);
+  const long s = std::min((256 + groups - 1) / groups, (long)table_width * kPage / (4 * kTile));
+  return (int)std::max(1L, std::min(s, 32L));
 }
 
 extern "C" int k8sllm_kv8_prefill(void* out, long out_stride, const void* qkv, long qkv_stride, const int* cu, const int* ctx, const int* qb_seq,
@@ -394,7 +425,7 @@ extern "C" int k8sllm_kv8_prefill(void* out, long out_stride, const void* qkv, l
                                   float* part_o, float* part_ml, hipStream_t s) {
   if (n_qblocks <= 0 || rows <= 0) return 0;
   if (Hq % Hkv || S < 1 || S > 32) return -2;
-  const int G = Hq / Hkv, Z = (128 * G + 255) / 256;
+  const int G = Hq / Hkv, Z = prefill_z(rows, G);
   const Kv8Prefill a{(bf16_t*)out, out_stride, (const bf16_t*)qkv, qkv_stride, cu, ctx, qb_seq, qb_start, (const uint8_t*)k, (const uint8_t*)v,
                      scales, pages, table, table_stride, table_width, rows, seqs, Hq, Hkv, G, Z, S, scale * 1.4426950408889634f, part_o, part_ml};
   const dim3 grid(Hkv, n_qblocks * Z, S);
