@@ -61,6 +61,8 @@ def rope_and_cache_kv8(qkv: torch.Tensor, positions: torch.Tensor, cos_sin: torc
     split-K slabs [nslabs, T, (Hq + 2 Hkv) * D]."""
     T = qkv.shape[0]
     if partial is not None:
+        if qkv.shape[1] != (Hq + 2 * Hkv) * D or not qkv.is_contiguous() or not 1 <= nslabs or partial.numel() < nslabs * qkv.numel():
+            raise ValueError("rope_and_cache_kv8: partial must hold nslabs x [T, (Hq + 2 Hkv) * D], qkv be contiguous rows of that many columns")
         reduce_slabs(partial, nslabs, T, (Hq + 2 * Hkv) * D, qkv.dtype, out=qkv)
     if apply_rope:
         rope_and_cache(qkv, positions, cos_sin, None, None, None, Hq, Hkv, D, True)
@@ -92,7 +94,7 @@ def paged_decode_fused_kv8(slabs: torch.Tensor, nslabs: int, positions: torch.Te
                            cache: KV8, block_tables: torch.Tensor, seq_lens: torch.Tensor, Hq: int, Hkv: int, D: int, scale: float,
                            workspace: Optional[tuple] = None, out: Optional[torch.Tensor] = None, splits: Optional[int] = None) -> torch.Tensor:
     """``paged_decode_fused`` over the 8-bit pages (D = 128): q / k / v of the new tokens are the sum of ``nslabs`` fp32 slabs [nslabs, B, (Hq + 2
-    Hkv) * D], rounded to bf16, q and k rotated at ``positions``; k, v go into the page of ``slot_mapping`` (which is the sequence's last one)
+    Hkv) * D], rounded to bf16, q and k rotated at ``positions`` (held to the ends of ``cos_sin``); k, v go into the page of ``slot_mapping`` (which is the sequence's last one)
     as ``rope_and_cache_kv8`` writes them, and attention is over what the pages then stand for, the new token's codes among them."""
     B = seq_lens.shape[0]
     if not _gpu(slabs):

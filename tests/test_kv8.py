@@ -139,12 +139,12 @@ def filled(gen, dev, lens, hkv, d, spare=2, spread=1.0):
     slots = torch.cat([table[i, :need[i]].repeat_interleave(16)[:n] * 16 + torch.arange(n, dtype=torch.int32) % 16 for i, n in enumerate(lens)])
     if T:
         qkv = torch.cat([torch.zeros(T, hkv, d, dtype=torch.bfloat16), rows], 1).reshape(T, -1).to(dev)
-        ops.rope_and_cache_kv8(qkv, None_positions(T, dev), table_of(d, dev), cache, slots.to(dev), hkv, hkv, d, apply_rope=False)
+        ops.rope_and_cache_kv8(qkv, no_positions(T, dev), table_of(d, dev), cache, slots.to(dev), hkv, hkv, d, apply_rope=False)
         book.write(slots, rows[:, :hkv].double(), rows[:, hkv:].double())
     return cache, table, book
 
 
-def None_positions(T, dev):
+def no_positions(T, dev):
     return torch.zeros(T, dtype=torch.int32, device=dev)
 
 
@@ -186,7 +186,7 @@ def test_write_whole_ragged_and_appended(dev, d, hkv):
         x = (rand(gen, T, 3 * hkv, d, spread=1.0) * size).bfloat16()
         book = Book(bigger)
         sl = torch.tensor(slots, dtype=torch.int32)
-        ops.rope_and_cache_kv8(x.reshape(T, -1).to(dev), None_positions(T, dev), table_of(d, dev), bigger, sl.to(dev), hkv, hkv, d, apply_rope=False)
+        ops.rope_and_cache_kv8(x.reshape(T, -1).to(dev), no_positions(T, dev), table_of(d, dev), bigger, sl.to(dev), hkv, hkv, d, apply_rope=False)
         book.write(sl, x[:, hkv:2 * hkv].double(), x[:, 2 * hkv:].double())
         book.check(bigger)
 
@@ -205,7 +205,7 @@ def test_write_every_magnitude(dev):
     cache = ops.kv8_cache(len(edge), hkv, d, device=dev)
     book = Book(cache)
     slots = torch.arange(T, dtype=torch.int32)
-    ops.rope_and_cache_kv8(x.reshape(T, -1).to(dev), None_positions(T, dev), table_of(d, dev), cache, slots.to(dev), 1, hkv, d, apply_rope=False)
+    ops.rope_and_cache_kv8(x.reshape(T, -1).to(dev), no_positions(T, dev), table_of(d, dev), cache, slots.to(dev), 1, hkv, d, apply_rope=False)
     book.write(slots, x[:, 1:2].double(), x[:, 2:].double())
     book.check(cache)
 
@@ -220,7 +220,7 @@ def test_write_numbers_that_are_not_finite(dev):
     cache = ops.kv8_cache(3, hkv, d, device=dev)
     book = Book(cache)
     slots = torch.arange(16, 36, dtype=torch.int32)
-    ops.rope_and_cache_kv8(x.reshape(20, -1).to(dev), None_positions(20, dev), table_of(d, dev), cache, slots.to(dev), hkv, hkv, d, apply_rope=False)
+    ops.rope_and_cache_kv8(x.reshape(20, -1).to(dev), no_positions(20, dev), table_of(d, dev), cache, slots.to(dev), hkv, hkv, d, apply_rope=False)
     book.write(slots, x[:, hkv:2 * hkv].double(), x[:, 2 * hkv:].double())
     book.check(cache)
     assert int(Book(cache).codes[0].isnan().sum()) == 2 + d
@@ -236,7 +236,7 @@ def test_write_leaves_everything_else(dev):
     before = [t.clone().view(torch.uint8).cpu() for t in (cache.k, cache.v)]
     x = rand(gen, 6, 3 * hkv, d).bfloat16()
     slots = torch.tensor([-1, 80, 1 << 30, 33, 34, -5], dtype=torch.int32)
-    ops.rope_and_cache_kv8(x.reshape(6, -1).to(dev), None_positions(6, dev), table_of(d, dev), cache, slots.to(dev), hkv, hkv, d, apply_rope=False)
+    ops.rope_and_cache_kv8(x.reshape(6, -1).to(dev), no_positions(6, dev), table_of(d, dev), cache, slots.to(dev), hkv, hkv, d, apply_rope=False)
     k, v = (t.view(torch.uint8).cpu() for t in (cache.k, cache.v))
     others = [0, 1, 3, 4]
     assert torch.equal(k[others], before[0][others]) and torch.equal(v[others], before[1][others])
@@ -274,7 +274,7 @@ def test_write_refuses_rows_out_of_order_on_the_cpu():
     qkv = torch.zeros(3, 192, dtype=torch.bfloat16)
     for slots in ([1, 0, 2], [0, 2, 1], [0, 16, 1], [3, 3, 4], [0, 2, 3]):
         with pytest.raises(ValueError, match="follow one another"):
-            ops.rope_and_cache_kv8(qkv, None_positions(3, "cpu"), table_of(64, "cpu"), cache, torch.tensor(slots, dtype=torch.int32), 1, 1, 64,
+            ops.rope_and_cache_kv8(qkv, no_positions(3, "cpu"), table_of(64, "cpu"), cache, torch.tensor(slots, dtype=torch.int32), 1, 1, 64,
                                    apply_rope=False)
 
 
@@ -559,6 +559,82 @@ def test_cache_sizes():
         ops.kv8_cache(5, 3, 96)
 
 
+@pytest.mark.parametrize("dev", DEVICES)
+def test_calls_of_nothing(dev):
+    hq, hkv, d = 4, 2, 128
+    cache = ops.kv8_cache(2, hkv, d, device=dev)
+    i32 = lambda *s: torch.zeros(*s, dtype=torch.int32, device=dev)  # noqa: E731
+    cols = (hq + 2 * hkv) * d
+    none = torch.zeros(0, cols, dtype=torch.bfloat16, device=dev)
+    ops.rope_and_cache_kv8(none, i32(0), table_of(d, dev), cache, i32(0), hq, hkv, d)
+    assert ops.paged_decode_kv8(none, cache, i32(0, 1), i32(0), hq, hkv, d, 0.1).shape == (0, hq * d)
+    assert ops.paged_decode_fused_kv8(torch.zeros(1, 0, cols, device=dev), 1, i32(0), table_of(d, dev), i32(0), cache, i32(0, 1), i32(0), hq, hkv, d,
+                                      0.1).shape == (0, hq * d)
+    assert ops.flash_prefill_kv8(none, i32(1), i32(0), cache, i32(0, 1), hq, hkv, d, 0.1).shape == (0, hq * d)
+    x = torch.ones(3, cols, dtype=torch.bfloat16, device=dev)
+    ops.rope_and_cache_kv8(x, i32(3), table_of(d, dev), cache, i32(3) - 1, hq, hkv, d, apply_rope=False)
+    assert all(int(t.view(torch.uint8).sum()) == 0 for t in (cache.k, cache.v)) and float(cache.scales.sum()) == 0
+
+
+@pytest.mark.gpu
+def test_offsets_past_32_bits():
+    """A cache of 4.4 GB of key codes: pages in its last part, whose byte offsets need 33 bits."""
+    hq, hkv, d, dev = 4, 2, 128, "cuda"
+    n = 1_100_000
+    gen = torch.Generator().manual_seed(51)
+    cache = ops.kv8_cache(n, hkv, d, device=dev)
+    L = 40
+    pages = [n - 1, 5, n - 77]
+    table = torch.tensor([pages], dtype=torch.int32)
+    slots = torch.tensor([pages[t // 16] * 16 + t % 16 for t in range(L)], dtype=torch.int32)
+    x = torch.round(torch.randn(L, hq + 2 * hkv, d, generator=gen) * 16) / 16
+    small = ops.kv8_cache(3, hkv, d)
+    book = Book(small)
+    near = torch.arange(L, dtype=torch.int32)
+    book.write(near, x[:, hq:hq + hkv].double(), x[:, hq + hkv:].double())
+    rows = x.bfloat16().view(L, -1).to(dev)
+    ops.rope_and_cache_kv8(rows[:-1], no_positions(L - 1, dev), table_of(d, dev), cache, slots[:-1].to(dev), hq, hkv, d, apply_rope=False)
+    cs = torch.cat([torch.ones(64, d // 2), torch.zeros(64, d // 2)], 1).to(dev)
+    pos = torch.tensor([L - 1], dtype=torch.int32, device=dev)
+    args = (hq, hkv, d, 2.0 ** -4)
+    got = ops.paged_decode_fused_kv8(x[-1:].reshape(1, 1, -1).to(dev), 1, pos, cs, slots[-1:].to(dev), cache, table.to(dev), pos + 1, *args)
+    at = torch.tensor(pages, device=dev)
+    book.check(ops.KV8(*(t.view(torch.uint8)[at].view(kv8.E4M3) if t.dtype == kv8.E4M3 else t[at] for t in cache)))
+    k, v = book.tokens([0, 1, 2], L)
+    check_attention(got, *attend(x[-1:, :hq].double(), k, v, args[3], L - 1))
+    check_attention(ops.paged_decode_kv8(rows[-1:], cache, table.to(dev), pos + 1, *args), *attend(x[-1:, :hq].double(), k, v, args[3], L - 1))
+    got = ops.flash_prefill_kv8(rows, torch.tensor([0, L], dtype=torch.int32, device=dev), torch.zeros(1, dtype=torch.int32, device=dev), cache,
+                                table.to(dev), *args)
+    check_attention(got, *attend(x[:, :hq].double(), k, v, args[3], 0))
+
+
+@pytest.mark.gpu
+def test_prefill_in_a_graph_with_its_splits():
+    """A captured chunk whose keys are split: the partials lie in the graph's own memory, every replay answers for the tokens of its time."""
+    hq, hkv, d = 8, 2, 128
+    gen = torch.Generator().manual_seed(61)
+    ctx, new = 1200, 30
+    cache, table, book = filled(gen, "cuda", [ctx + new], hkv, d)
+    q = torch.zeros(new, hq * d, dtype=torch.bfloat16, device="cuda")
+    cu, cs, tb = torch.tensor([0, new], dtype=torch.int32).cuda(), torch.tensor([ctx], dtype=torch.int32).cuda(), table.cuda()
+    qb = (torch.zeros(1, dtype=torch.int32).cuda(), torch.zeros(1, dtype=torch.int32).cuda())
+    run = lambda: ops.flash_prefill_kv8(q, cu, cs, cache, tb, hq, hkv, d, 0.1, qblocks=qb)  # noqa: E731
+    run()
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        out = run()
+    for _ in range(3):
+        x = rand(gen, new, hq, d).bfloat16()
+        q.copy_(x.view(new, -1))
+        g.replay()
+        torch.cuda.synchronize()
+        other = run()
+        want = attend(x.double(), *book.tokens(table[0], ctx + new), 0.1, ctx)
+        check_attention(out, *want)
+        check_attention(other, *want)
+
+
 @pytest.mark.gpu
 def test_refusals():
     """Arguments that the kernels do not take are errors on the host."""
@@ -588,6 +664,7 @@ def test_refusals():
              (dec, dict(cache=ops.KV8(cache.k, cache.v, cache.scales[:2]))), (dec, dict(Hq=64)),
              (pre, dict(ctx_start=i32(0))), (pre, dict(block_tables=table[:1])), (pre, dict(scale=math.inf)), (pre, dict(out=q[:1])),
              (wr, dict(slot_mapping=i32(0))), (wr, dict(qkv=qkv[:, : hq * d])), (wr, dict(slot_mapping=i32(0, 1).long())),
+             (wr, dict(partial=torch.zeros(2 * 8 * 128, device=dev), nslabs=2)),
              (wr, dict(cache=ops.KV8(cache.k.cpu(), cache.v, cache.scales))),
              (fus, dict(nslabs=2)), (fus, dict(nslabs=0)), (fus, dict(positions=i32(2))), (fus, dict(cos_sin=cs[:, :64])),
              (fus, dict(slabs=slabs.bfloat16())), (fus, dict(slot_mapping=i32(1)))]
