@@ -22,9 +22,9 @@
 // waves have read their pages, writes them; if the page's scale grows it rounds the earlier tokens' codes anew, for its own products too: the
 // answer is that of the write and the attention one after the other.
 //
-// Bound by memory: 64 x ~1.7 k tokens, 8 kv heads, 231 MB: 43 us, 5.3 TB/s (the same kernel without its products 41; a large sum reads 6.0);
-// 8 x 31 k tokens, 512 MB: 93 us; over the bf16 cache the first takes 79 us.  One sequence of 1.7 k tokens: 10 us, of which a launch is 3 to
-// 4, each trip to memory in the chain of lengths, pages, codes and partials near 1.
+// Bound by memory: 64 x ~1.7 k tokens, 8 kv heads, 231 MB: 43 us, 5.3 TB/s (the same kernel without its products 41 to 43; a large sum reads 6.0);
+// 8 x 31 k tokens, 512 MB: 93 us; over the bf16 cache the first takes 79 us.  One sequence of 1.7 k tokens: 10 us, of one token 6.9,
+// a launch that does nothing 3 to 4.
 #include "kv8.h"
 
 namespace k8sllm {

@@ -9,7 +9,7 @@
 //
 // Scores are v_mfma_scale_f32_32x32x64_f8f6f4 on the codes as they lie, with the page's scale as the operand's: K is staged without a
 // conversion and read from LDS at half the bytes.  q is the sum of two e4m3 numbers (see there), so nothing of bf16's precision is lost; two
-// products at twice the rate cost what one in bf16 does.  (In bf16, K converted on its way: 908 us for the last figure below, 825 so.)
+// products at twice the rate cost what one in bf16 does.  (In bf16, K converted on its way: 908 us for the first figure below, 835 so.)
 // Probabilities as two e4m3 numbers would spare V's conversion but cost more in vector instructions than it does.
 //
 // Tiles of 64 keys (4 pages).  A thread loads 16 bytes of K codes and 16 of V codes a tile, a tile ahead of their way into LDS, where V
@@ -17,8 +17,8 @@
 // that.  Staging goes between the wave's score products.  Four buffers of 24 KB (D = 128) and a barrier every other tile: waves drift apart by
 // up to two tiles, and the second half of a tile - exponentials and the second product, both units at work - has priority over another
 // wave's first, so that the two waves of a SIMD are in different halves more often than not (a barrier a tile, or no priority: 828 and
-// 835 us for 807).  Bound by MFMAs, LDS reads and exponentials in about equal parts: a tile's 32 and 64 KB of the eight waves' reads
-// and 2 x 1000 cycles of vector instructions take 2000 cycles each.
+// 835 us for 807).  No unit alone bounds it: MFMAs are busy 56 % of the time and the vector
+// units 61 %, LDS conflicts are 5 % (counters, 4096 rows behind 12 k).
 //
 // A V code that is NaN counts for rows that see its token and no others, though all rows of a tile multiply it (0 * NaN): the tile is
 // staged with zero in its place, and the first such token of each dim is kept and put on the rows behind it at the end.
@@ -26,8 +26,8 @@
 // Few rows (a short question behind a long conversation) leave most of the chip idle: the keys are then split S ways and fp32 partials
 // joined by a second launch.
 //
-// Measured: 4096 rows behind 12 k tokens, 32 heads over 8: 807 us, 1.19 PFLOP/s (a large bf16 library product: 1.36); 10 x 1124 rows behind 512: 222 us,
-// 0.80; 45 rows behind 4 k tokens: 23 us.
+// Measured: 4096 rows behind 12 k tokens, 32 heads over 8: 807 to 859 us on two boxes, 1.12 to 1.19 PFLOP/s (a large bf16 library product: 1.36); 10 x up to 1124 rows
+// behind 512: 222 to 234 us, 0.76 to 0.81; 45 rows behind 4 k tokens: 23 us.
 #include <algorithm>
 
 #include "kv8.h"

@@ -8,7 +8,7 @@
 //
 // Magnitudes are compared as the 16-bit patterns that they are, two to an instruction, and v_cvt_scalef32_pk_fp8_bf16 takes packed bf16 and the
 // scale: about 130 instructions a run (in 32-bit arithmetic 1000, which took longer than the memory: 28 us for the figure below).
-// Bound by memory at prefill: per row and kv head 4 D bytes in, 2 D out; 16384 rows x 8 heads x 128 dims, 100 MB: 20.9 us, 4.8 TB/s (a large copy
+// Bound by memory at prefill: per row and kv head 4 D bytes in, 2 D out; 16 k rows x 8 heads x 128 dims, 98 MB: 19.3 us, 5.1 TB/s (a large copy
 // moves 5.1).
 #include "kv8.h"
 
