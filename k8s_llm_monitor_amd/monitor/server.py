@@ -600,11 +600,14 @@ def _chat_controls(d: dict) -> dict:
         if d.get(k) is not None:
             if not isinstance(d[k], (int, float)) or isinstance(d[k], bool):
                 raise http_error(400, f"{k} must be a number")
-            c[k] = float(d[k])
+            try:
+                c[k] = float(d[k])
+            except OverflowError:  # a whole number of hundreds of digits
+                raise http_error(400, f"{k} is too large") from None
     if d.get("logit_bias"):
         try:
             c["logit_bias"] = {int(t): float(x) for t, x in d["logit_bias"].items()}
-        except (AttributeError, TypeError, ValueError):
+        except (AttributeError, TypeError, ValueError, OverflowError):
             raise http_error(400, "logit_bias must map token ids to numbers") from None
     return c
 

@@ -17,6 +17,7 @@ from . import _gpu, native
 
 PAGE = 16
 MAX_BIAS = 2046  # biased tokens a slot
+LARGEST = 1e30  # of a penalty or a finite bias
 
 
 class LogitControls(NamedTuple):
@@ -53,15 +54,15 @@ class LogitControls(NamedTuple):
 
 
 def check_controls(repetition: float = 1.0, presence: float = 0.0, frequency: float = 0.0, bias: Optional[dict] = None) -> None:
-    """ValueError for controls without a meaning."""
+    """ValueError for controls without a meaning, or so large that sums of them would pass 32 bits (2^20 times a frequency penalty is the most)."""
     import math
-    if not (repetition > 0 and math.isfinite(repetition)):
-        raise ValueError(f"repetition penalty {repetition}: a positive number")
-    if not (math.isfinite(presence) and math.isfinite(frequency)):
-        raise ValueError(f"presence {presence} and frequency {frequency}: finite numbers")
+    if not 1 / LARGEST <= repetition <= LARGEST:
+        raise ValueError(f"repetition penalty {repetition}: a positive number, {1 / LARGEST} to {LARGEST}")
+    if not (abs(presence) <= LARGEST and abs(frequency) <= LARGEST):
+        raise ValueError(f"presence {presence} and frequency {frequency}: numbers up to {LARGEST}")
     for t, x in (bias or {}).items():
-        if int(t) != t or t < 0 or math.isnan(float(x)):
-            raise ValueError(f"bias {x!r} of token {t!r}: token ids and numbers")
+        if int(t) != t or t < 0 or not (abs(float(x)) <= LARGEST or math.isinf(x)):
+            raise ValueError(f"bias {x!r} of token {t!r}: token ids and numbers up to {LARGEST}, or infinite")
 
 
 def allowed_mask(allowed: Iterable[int], vocab: int) -> torch.Tensor:

@@ -232,3 +232,11 @@ def test_chat_requests_have_them():
     assert err.value.code == 400
     Backend.takes_controls = False
     assert text(ask(frequency_penalty=0.5)) == "null"
+
+
+@pytest.mark.parametrize("field", [{"presence_penalty": 10 ** 400}, {"logit_bias": {"1": -10 ** 400}}])
+def test_chat_numbers_of_hundreds_of_digits_are_bad_requests(field):
+    from k8s_llm_monitor_amd.monitor.server import _chat_controls
+    with pytest.raises(Exception) as err:
+        _chat_controls(json.loads(json.dumps(field)))
+    assert err.value.code == 400

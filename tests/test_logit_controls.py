@@ -191,6 +191,16 @@ def test_refused_controls():
     assert c.info.tolist() == [[0, 0], [0, 0]]
 
 
+@pytest.mark.parametrize("bad", [dict(repetition=1e-50), dict(repetition=1e39), dict(presence=1e39), dict(frequency=-1e39), dict(frequency=3e38),
+                                 dict(bias={1: 1e39}), dict(bias={1: -3e38})])
+def test_controls_that_32_bits_do_not_hold_are_refused(bad):
+    """Finite numbers that are infinite or zero in 32 bits, or whose sums are: rows would hold NaN."""
+    c = ops.logit_controls(1, 100, 3)
+    with pytest.raises(ValueError):
+        c.set(0, 5, **bad)
+    c.set(0, 5, presence=-1e30, bias={1: -math.inf, 2: math.inf, 3: 1e30})
+
+
 @pytest.mark.gpu
 def test_refused_calls():
     dev, B, V = "cuda", 2, 300
