@@ -110,7 +110,9 @@ __device__ int sample_row_filtered(const T* __restrict__ x, int V, float temp, i
   if (mn > mx) k = 0, p = 1.f;  // every token masked: nothing to filter
   float thr = -INFINITY;
   if (k > 0 && k < V) {
-    float lo = mn, hi = mx;  // invariant: count(x >= lo) >= k
+    // invariant: count(x >= lo) >= k.  A finite logit far below the others (a bias of -1e30) would leave the halvings too coarse to part the rest:
+    // there the search is over the last 80, below which no noise (19.5 at most between two tokens) makes a token win
+    float lo = mx - mn > 4096.f ? mx - 80.f : mn, hi = mx;
     for (int it = 0; it < 26; ++it) {
       const float mid = 0.5f * (lo + hi);
       float c = 0.f;

@@ -178,6 +178,23 @@ def test_sampling_behind_a_mask(dev, top_k, top_p):
         assert dev == "cpu" or t[4] == 0
 
 
+@pytest.mark.parametrize("dev", DEVICES)
+@pytest.mark.parametrize("far", [-1e4, -1e30])
+def test_top_k_behind_a_far_bias(dev, far):
+    """A token biased far below the others does not widen what top-k keeps, neither do many."""
+    V = 5000
+    x = torch.randn(2, V, generator=torch.Generator().manual_seed(9)).to(dev)
+    y = x.clone()
+    y[0, 7] = far
+    y[1, 3:] = far  # three tokens left of five: the others have probability zero
+    best = [set(y[0].topk(5).indices.tolist()), {0, 1, 2}]
+    full = lambda v, t: torch.full((2,), v, dtype=t, device=dev)  # noqa: E731
+    rng = torch.tensor([4, 0], dtype=torch.int64, device=dev)
+    for _ in range(40):
+        t = ops.sample(y, full(1.0, torch.float32), full(5, torch.int32), full(1.0, torch.float32), rng, advance=True).tolist()
+        assert t[0] in best[0] and t[1] in best[1]
+
+
 def test_refused_controls():
     c = ops.logit_controls(2, 100, 3)
     for bad in (dict(repetition=0.0), dict(repetition=math.nan), dict(presence=math.inf), dict(frequency=math.nan), dict(bias={-1: 1.0}),
