@@ -413,6 +413,7 @@ static int prefill_z(int rows, int G) { return (std::min(128, rows) * G + 255) /
 // that the block tables allow.  (A split's partials are 512 bytes a row and head out and in: 45 rows behind 4 k tokens, 32 heads: 16 splits
 // of 5 tiles 17.5 + 4.0 us, 32 of 3 tiles 17.4 + 5.5.)
 extern "C" int k8sllm_kv8_prefill_splits(int n_qblocks, int rows, int Hq, int Hkv, int table_width) {
+  if (rows > 128L * n_qblocks) return 1;  // rows that no q-block names: partials are of all rows, and few of many would ask for gigabytes
   const int G = Hq / Hkv, Z = prefill_z(rows, G);
   const long groups = std::max(1L, std::min((long)n_qblocks * Z, (long)rows * G / 256 + n_qblocks) * Hkv);
   const long s = std::min((256 + groups - 1) / groups, (long)table_width * kPage / (4 * kTile));

@@ -672,3 +672,27 @@ def test_refusals():
         with pytest.raises((RuntimeError, ValueError)):
             f(**k)
     torch.cuda.synchronize()
+
+
+@pytest.mark.gpu
+def test_prefill_of_few_named_rows_takes_little_memory():
+    """One q-block of many rows: right for its rows, the others left as they are, and no partials for rows that nothing names."""
+    hq, hkv, d, dev = 8, 2, 128, "cuda"
+    gen = torch.Generator().manual_seed(71)
+    ctx, new, T = 2000, 40, 4096
+    cache, table, book = filled(gen, dev, [ctx + new], hkv, d)
+    x = rand(gen, new, hq, d).bfloat16()
+    q = torch.zeros(T, hq * d, dtype=torch.bfloat16, device=dev)
+    q[:new] = x.view(new, -1)
+    out = torch.full((T, hq * d), 7.0, dtype=torch.bfloat16, device=dev)
+    i32 = lambda *v: torch.tensor(v, dtype=torch.int32, device=dev)  # noqa: E731
+    args = (i32(0, new), i32(ctx), cache, table.to(dev), hq, hkv, d, 0.1)
+    qb = (i32(0), i32(0))
+    torch.cuda.synchronize()
+    torch.cuda.reset_peak_memory_stats()
+    before = torch.cuda.memory_allocated()
+    ops.flash_prefill_kv8(q, *args, qblocks=qb, out=out)
+    torch.cuda.synchronize()
+    assert torch.cuda.max_memory_allocated() == before
+    check_attention(out[:new], *attend(x.double(), *book.tokens(table[0], ctx + new), 0.1, ctx))
+    assert bool((out[new:] == 7).all())
