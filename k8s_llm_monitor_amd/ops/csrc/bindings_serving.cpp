@@ -116,6 +116,7 @@ void kv8_write(Tensor qkv, Tensor slots, Tensor k, Tensor v, Tensor scales, int6
   c.whole(slots, torch::kInt32, "slot_mapping");
   const int64_t T = qkv.size(0);
   TORCH_CHECK(slots.numel() >= T && T < (1LL << 30), c.what, ": a slot for each row");
+  TORCH_CHECK(T * Hkv < (1LL << 31), c.what, ": rows times kv heads below 2^31");  // waves are numbered in 32 bits
   c.done(k8sllm_kv8_write(qkv.data_ptr(), qkv.stride(0), slots.data_ptr<int>(), cache.k, cache.v, cache.scales, (int)T, h.Hq, h.Hkv, h.D,
                           cache.pages, c.stream()));
 }
@@ -181,7 +182,7 @@ void kv8_decode_fused(Tensor out, Tensor slabs, int64_t nslabs, Tensor positions
   c.whole(cos_sin, torch::kFloat32, "cos_sin");
   c.whole(slabs, torch::kFloat32, "slabs");
   const int64_t B = lens.numel();
-  TORCH_CHECK(nslabs >= 1 && slabs.numel() >= nslabs * B * (Hq + 2 * Hkv) * D && (uintptr_t)slabs.data_ptr() % 16 == 0, c.what,
+  TORCH_CHECK(nslabs >= 1 && nslabs < (1 << 20) && slabs.numel() >= nslabs * B * (Hq + 2 * Hkv) * D && (uintptr_t)slabs.data_ptr() % 16 == 0, c.what,
               ": slabs must hold nslabs x [B, (Hq + 2 Hkv) * D], from 16 bytes on");
   TORCH_CHECK(positions.numel() >= B && cos_sin.dim() == 2 && cos_sin.size(0) >= 1 && cos_sin.size(1) == D, c.what,
               ": positions [B] and cos_sin [positions, D]");
@@ -213,7 +214,7 @@ void kv8_prefill(Tensor out, Tensor qkv, Tensor cu, Tensor ctx, Tensor qb_seq, T
   const Cache cache(c, h, k, v, scales);
   const Table t(c, table, seqs);
   c.typed(out, torch::kBFloat16, "out");
-  TORCH_CHECK(out.dim() == 2 && out.size(0) >= T && out.size(1) == Hq * D && (T == 0 || out.stride(1) == 1) && (out.stride(0) % 4 == 0 || T <= 1) &&
+  TORCH_CHECK(out.dim() == 2 && out.size(0) >= T && out.size(1) == Hq * D && (T == 0 || out.stride(1) == 1) && ((out.stride(0) % 4 == 0 && out.stride(0) >= Hq * D) || T <= 1) &&
                   (uintptr_t)out.data_ptr() % 8 == 0, c.what, ": out must be [T, Hq * D], from 8 bytes on");
   TORCH_CHECK(nq * ((128 * (Hq / Hkv) + 255) / 256) <= 65535 && T < (1LL << 30), c.what, ": too many q-blocks");
   if (T == 0 || nq == 0) return;
@@ -239,6 +240,7 @@ void logit_controls(Tensor out, Tensor logits, Tensor params, Tensor info, Tenso
               ": logits bfloat16 or float32, out of the same type or float32");
   TORCH_CHECK(out.is_cuda() && out.get_device() == c.dev, c.what, ": out must be on the same GPU");
   TORCH_CHECK(B == 0 || V == 0 || (logits.stride(1) == 1 && out.stride(1) == 1 && V < (1LL << 30)), c.what, ": rows must be contiguous");
+  TORCH_CHECK(B <= 1 || out.stride(0) >= V, c.what, ": rows of out must not overlap");
   TORCH_CHECK(B <= 65535, c.what, ": at most 65535 rows");
   if (B == 0 || V == 0) return;
   c.whole(params, torch::kFloat32, "controls.params");

@@ -696,3 +696,26 @@ def test_prefill_of_few_named_rows_takes_little_memory():
     assert torch.cuda.max_memory_allocated() == before
     check_attention(out[:new], *attend(x.double(), *book.tokens(table[0], ctx + new), 0.1, ctx))
     assert bool((out[new:] == 7).all())
+
+
+@pytest.mark.gpu
+def test_refused_sizes_and_overlapping_rows():
+    """Products of sizes past 32 (or 64) bits, and outputs whose rows share memory, are errors on the host."""
+    dev, hq, hkv, d = "cuda", 2, 2, 128
+    i32 = lambda *v: torch.tensor(v, dtype=torch.int32, device=dev)  # noqa: E731
+    cache, cs = ops.kv8_cache(4, hkv, d, device=dev), table_of(d, dev)
+    wide = ops.kv8_cache(1, 4096, 64, device=dev)
+    rows = torch.zeros(1, 3 * 4096 * 64, dtype=torch.bfloat16, device=dev).expand(1 << 19, -1)
+    with pytest.raises(RuntimeError, match="2.31"):
+        ops.rope_and_cache_kv8(rows, None, None, wide, torch.full((1 << 19,), -1, dtype=torch.int32, device=dev), 4096, 4096, 64, apply_rope=False)
+    slabs, table, lens = torch.zeros(1, 2, 3 * hq * d, device=dev), torch.zeros(2, 2, dtype=torch.int32, device=dev), i32(3, 4)
+    with pytest.raises(RuntimeError, match="nslabs"):
+        ops.paged_decode_fused_kv8(slabs, 1 << 60, i32(2, 3), cs, i32(2, 3), cache, table, lens, hq, hkv, d, 0.1)
+    q = torch.zeros(2, hq * d, dtype=torch.bfloat16, device=dev)
+    with pytest.raises(RuntimeError, match="out must be"):
+        ops.flash_prefill_kv8(q, i32(0, 1, 2), i32(0, 0), cache, table, hq, hkv, d, 0.1, out=q[:1].expand(2, -1))
+    c = ops.logit_controls(1, 64, 2, device=dev)
+    with pytest.raises(RuntimeError, match="overlap"):
+        ops.control_logits(torch.zeros(2, 64, device=dev), c, i32(0, 0), torch.zeros(1, 16, dtype=torch.int32, device=dev), table, lens,
+                           out=torch.zeros(1, 64, device=dev).expand(2, -1))
+    torch.cuda.synchronize()
