@@ -233,7 +233,9 @@ class ModelRunner:
         cu[1:] = np.cumsum(lens)
         qs, st = ops.prefill_qblocks(cu.tolist(), ctx_starts=starts)
         nq = len(qs)
-        paged = any(starts) or (self.hybrid and bool(seqs))  # layer-list attention always reads the pages
+        # layer-list attention and the 8-bit cache's always read the pages: there a prompt's answer hangs neither on its neighbours in the
+        # step nor on where it is cut
+        paged = any(starts) or ((self.hybrid or self.kv8) and bool(seqs))
         W = max(len(s.block_table) for s in seqs) if paged else 0
         Wd = max(len(q.block_table) for q in decode) if nd else 0
         # TP > 1: two micro-batches of whole sequences, so one's row-parallel all-reduces overlap

@@ -353,7 +353,9 @@ class CausalLM:
                 paged = (meta.ctx_start, k_cache, v_cache, meta.block_tables)
 
             def prefill(rows, out=None):
-                if kv8 is not None and paged is not None:  # (whole prompts attend their own rows, which are at hand in full)
+                if kv8 is not None:  # from the pages, whole prompts too: they stand for the same numbers in every step
+                    if paged is None:
+                        raise ValueError("a prefill step over the 8-bit cache needs ctx_start and block_tables")
                     return ops.flash_prefill_kv8(rows, meta.cu_seqlens, meta.ctx_start, kv8, meta.block_tables, self.hq, self.hkv,
                                                  self.D, self.scale, qblocks=qb, out=out)
                 return ops.flash_prefill(rows, meta.cu_seqlens, self.hq, self.hkv, self.D, self.scale, qblocks=qb,

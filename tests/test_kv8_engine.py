@@ -240,3 +240,60 @@ def test_chat_numbers_of_hundreds_of_digits_are_bad_requests(field):
     with pytest.raises(Exception) as err:
         _chat_controls(json.loads(json.dumps(field)))
     assert err.value.code == 400
+
+
+# ---------------------------------------------------------------- one rule for every prompt
+
+def first_logits(e, s, steps=40):
+    """The logits that a prompt's first token is taken from."""
+    for _ in range(steps):
+        e.step()
+        if s.output_ids:
+            return e.runner.last_logits[-1].float().cpu().clone()
+    raise AssertionError("no token")
+
+
+def held_codes(e, s, n):
+    """The key codes of a sequence's first n tokens, every layer."""
+    pages = torch.tensor(s.block_table[: n // 16])
+    return e.runner.k_cache.view(torch.uint8)[:, pages.to(e.runner.k_cache.device)].cpu()
+
+
+def test_a_prompt_answers_alike_alone_beside_others_and_in_chunks():
+    """fp32 rows: beside a prompt whose prefix is cached, and cut into chunks (at a page's border and inside one), a prompt's logits and pages are
+    what they are alone.  The matrix products' row counts differ, so rows do by a few steps of 2^-24, and now and then a code whose value lies that near
+    to the middle of two (of a thousand codes fewer than one); 2^-10 of the norm is far above both, and thirty times below what attending unrounded rows makes."""
+    kw = dict(kv_cache_dtype="fp8", keep_logits=True, pipeline=False)
+    p, shared = prompt(60, 7), prompt(64, 8)
+    par = SamplingParams(max_tokens=4, **GREEDY)
+    got = []
+    for how in ("alone", "beside", "chunks of 48", "chunks of 40"):
+        e = engine("cpu", **kw, **({"max_prefill_tokens": int(how[-2:])} if how[:6] == "chunks" else {}))
+        if how == "beside":
+            drain(e, [e.add_request(shared + prompt(3, 9), par)])
+            e.add_request(shared + prompt(30, 10), par)
+        s = e.add_request(p, par)
+        got.append((first_logits(e, s), held_codes(e, s, len(p))))
+        if how == "beside":
+            assert e.runner.n_steps["prefill_context_tokens"] >= 64
+    for logits, codes in got[1:]:
+        assert float((logits - got[0][0]).norm() / got[0][0].norm()) <= 2.0 ** -10
+        assert float((codes != got[0][1]).float().mean()) <= 1e-3
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+def test_whole_prompts_attend_the_pages(dev, monkeypatch):
+    """No step over the 8-bit cache attends unrounded rows; a step without block tables is refused."""
+    from k8s_llm_monitor_amd import ops
+    from k8s_llm_monitor_amd.models.llama import AttnMeta
+    e = engine(dev, kv_cache_dtype="fp8")
+    calls = []
+    whole, pages = ops.flash_prefill, ops.flash_prefill_kv8
+    monkeypatch.setattr(ops, "flash_prefill", lambda *a, **k: calls.append("rows") or whole(*a, **k))
+    monkeypatch.setattr(ops, "flash_prefill_kv8", lambda *a, **k: calls.append("pages") or pages(*a, **k))
+    drain(e, [e.add_request(prompt(n, n), SamplingParams(max_tokens=3, **GREEDY)) for n in (1, 20, 70)])
+    assert calls and set(calls) == {"pages"}
+    i32 = lambda *v: torch.tensor(v, dtype=torch.int32, device=e.runner.device)  # noqa: E731
+    meta = AttnMeta(is_prefill=True, positions=i32(0, 1), slot_mapping=i32(-1, -1), cu_seqlens=i32(0, 2), logits_idx=i32(1).long())
+    with pytest.raises(ValueError, match="block_tables"):
+        e.model.forward(i32(5, 6), meta, e.runner.kv)
