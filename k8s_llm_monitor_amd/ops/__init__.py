@@ -851,6 +851,10 @@ def _sample_cpu(logits, temperature, top_k, top_p, rng):
             res[b] = int(x.argmax())
             continue
         x = x / t
+        top = float(x.max())
+        if math.isinf(top):  # no distribution to draw from: the first of the infinite ones, of a row of nothing but -inf the first token
+            res[b] = int((x == top).nonzero()[0])
+            continue
         if top_k is not None and 0 < int(top_k[b]) < x.numel():
             kth = torch.topk(x, int(top_k[b])).values[-1]
             x = x.masked_fill(x < kth, float("-inf"))

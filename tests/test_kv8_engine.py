@@ -297,3 +297,13 @@ def test_whole_prompts_attend_the_pages(dev, monkeypatch):
     meta = AttnMeta(is_prefill=True, positions=i32(0, 1), slot_mapping=i32(-1, -1), cu_seqlens=i32(0, 2), logits_idx=i32(1).long())
     with pytest.raises(ValueError, match="block_tables"):
         e.model.forward(i32(5, 6), meta, e.runner.kv)
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+@pytest.mark.parametrize("top_p", [1.0, 0.9])
+def test_an_infinite_bias_beside_an_ordinary_request(dev, top_p):
+    """Sampled at a temperature: the biased row takes its token at every step, the other request finishes."""
+    e = engine(dev, logit_controls=True)
+    par = dict(max_tokens=6, temperature=0.7, top_p=top_p, ignore_eos=True)
+    got = drain(e, [e.add_request(prompt(20, 1), SamplingParams(logit_bias={7: float("inf")}, **par)), e.add_request(prompt(30, 2), SamplingParams(**par))])
+    assert got[0] == [7] * 6 and len(got[1]) == 6

@@ -264,3 +264,23 @@ def test_replays_in_a_graph():
         torch.cuda.synchronize()
         old.view(-1)[[19, 34, 95]] = new
         check(out, *plain(xs, ctl, rows.tolist(), old, table.tolist(), lens.tolist()))
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+@pytest.mark.parametrize("top_k,top_p", [(0, 1.0), (3, 1.0), (0, 0.9), (50, 0.5)])
+@pytest.mark.parametrize("temp", [0.0, 0.7])
+def test_sampling_of_infinite_logits(dev, top_k, top_p, temp):
+    """Tokens of an infinite bias win, the lowest of several; a row of nothing but -inf gives token 0; an ordinary row beside them goes on."""
+    V = 700
+    x = torch.randn(4, V, generator=torch.Generator().manual_seed(3))
+    x[0, 77] = math.inf
+    x[1, 600], x[1, 9] = math.inf, math.inf
+    x[1, 10:500] = -math.inf
+    x[2] = -math.inf
+    x[3, :500] = -math.inf
+    x = x.to(dev)
+    full = lambda v, t: torch.full((4,), v, dtype=t, device=dev)  # noqa: E731
+    rng = torch.tensor([6, 0], dtype=torch.int64, device=dev)
+    for _ in range(10):
+        t = ops.sample(x, full(temp, torch.float32), full(top_k, torch.int32), full(top_p, torch.float32), rng, advance=True).tolist()
+        assert t[:3] == [77, 9, 0] and 500 <= t[3] < V
