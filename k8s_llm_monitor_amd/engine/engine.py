@@ -199,6 +199,9 @@ class LLMEngine:
         ids = list(bias) + list(p.allowed_token_ids or ())
         if any(int(t) != t or not 0 <= t < V for t in ids) or (p.allowed_token_ids is not None and not len(p.allowed_token_ids)):
             raise ValueError(f"logit_bias and allowed_token_ids: token ids below {V}, at least one allowed")
+        banned = {int(t) for t, x in bias.items() if x == float("-inf")}
+        if banned and banned.issuperset(map(int, p.allowed_token_ids if p.allowed_token_ids is not None else range(V))):
+            raise ValueError("logit_bias: every allowed token is biased to -inf")
 
     def has_work(self) -> bool:
         return self.sched.has_work() or self._inflight is not None or self._pf_inflight is not None

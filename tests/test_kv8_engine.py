@@ -307,3 +307,16 @@ def test_an_infinite_bias_beside_an_ordinary_request(dev, top_p):
     par = dict(max_tokens=6, temperature=0.7, top_p=top_p, ignore_eos=True)
     got = drain(e, [e.add_request(prompt(20, 1), SamplingParams(logit_bias={7: float("inf")}, **par)), e.add_request(prompt(30, 2), SamplingParams(**par))])
     assert got[0] == [7] * 6 and len(got[1]) == 6
+
+
+def test_requests_that_allow_no_token_are_refused():
+    e = engine("cpu", logit_controls=True)
+    out = float("-inf")
+    for bad in (dict(allowed_token_ids=(5,), logit_bias={5: out}), dict(allowed_token_ids=(5, 6, 5), logit_bias={5: out, 6: out, 9: 1.0})):
+        with pytest.raises(ValueError, match="allowed"):
+            e.add_request([5, 6], SamplingParams(**bad))
+    few = engine("cpu", logit_controls=True, max_logit_bias=2000)  # (the vocabulary has 1024)
+    with pytest.raises(ValueError, match="allowed"):
+        few.add_request([5, 6], SamplingParams(logit_bias=dict.fromkeys(range(few.model_cfg.vocab_size), out)))
+    s = e.add_request([5, 6], SamplingParams(max_tokens=3, temperature=0.9, ignore_eos=True, allowed_token_ids=(5, 6), logit_bias={5: out}))
+    assert drain(e, [s])[0] == [6] * 3
