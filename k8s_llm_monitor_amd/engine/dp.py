@@ -97,6 +97,8 @@ def _replica_main(conn, idx: int, cfg: dict, device: str) -> None:
                                 "replica": idx}))
         except (EngineOverloaded, EngineUnavailable) as e:
             send(("busy", key, str(e)))
+        except ValueError as e:  # a request that the engine refuses, as EngineService has it
+            send(("refused", key, str(e)))
         except BaseException as e:  # noqa: BLE001
             send(("fail", key, repr(e)))
 
@@ -229,7 +231,7 @@ class ReplicaRouter:
                     except Exception:  # noqa: BLE001 - a broken consumer must not stop the reader
                         pass
                 continue
-            if kind in ("done", "fail", "busy"):
+            if kind in ("done", "fail", "busy", "refused"):
                 with self._lock:
                     fut, _ = self._pending.pop(key, (None, None))
                     self._streams.pop(key, None)
@@ -246,6 +248,8 @@ class ReplicaRouter:
                     from .engine import EngineOverloaded
 
                     fut.set_exception(EngineOverloaded(f"replica {r.idx}: {body}"))
+                elif kind == "refused":
+                    fut.set_exception(ValueError(body))
                 else:
                     fut.set_exception(RuntimeError(f"replica {r.idx}: {body}"))
             elif kind == "stats":

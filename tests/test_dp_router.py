@@ -76,6 +76,40 @@ def test_server_assembly_with_dp_replicas(tmp_path):
         svc.close()
 
 
+def test_refused_requests_are_value_errors_behind_replicas():
+    """What an engine refuses is a ValueError through the router too - 400 at the chat endpoint - and the replica goes on."""
+    import json
+
+    from k8s_llm_monitor_amd.llm.service import LocalEngineBackend
+    from k8s_llm_monitor_amd.monitor.server import MonitorApp
+
+    cfg = EngineConfig(**CFG, logit_controls=True)
+    router = ReplicaRouter(cfg, ["cpu"])
+    try:
+        V = router.engine.model_cfg.vocab_size
+        for bad in (dict(logit_bias={V: 1.0}), dict(repetition_penalty=0.0), dict(presence_penalty=1e39)):
+            with pytest.raises(ValueError):
+                router.submit([5, 6], SamplingParams(**bad)).result(timeout=60)
+
+        class Analysis:
+            backend = LocalEngineBackend(router, max_tokens=2, temperature=0.0, timeout_s=60)
+
+            def fit_chat(self, parts, mt):
+                return "\n".join(parts)
+
+        app = MonitorApp.__new__(MonitorApp)
+        app.analysis = Analysis()
+        app._bounded = lambda fn: fn()
+        ask = lambda **k: app.chat_completions("POST", json.dumps({"messages": [{"role": "user", "content": "hi"}], **k}).encode(), {})  # noqa: E731
+        with pytest.raises(Exception) as err:
+            ask(logit_bias={str(V): 1})
+        assert err.value.code == 400
+        ok = router.submit([5, 6], SamplingParams(max_tokens=2, temperature=0.0, ignore_eos=True, logit_bias={7: 1e4})).result(timeout=60)
+        assert ok[1].output_ids == [7, 7]
+    finally:
+        router.close()
+
+
 @pytest.mark.gpu
 def test_gpu_router_two_replicas_share_one_gpu():
     """Two replica processes on cuda:0 (the box has one GPU): HIP kernels + hipGraph decode in
