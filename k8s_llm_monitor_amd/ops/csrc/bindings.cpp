@@ -15,7 +15,7 @@ int k8sllm_gelu_tanh(void* out, const void* x, long n, hipStream_t s);
 int k8sllm_embedding(void* out, const int* ids, const void* weight, long T, int d, int vocab_start, int rows,
                      hipStream_t s);
 int k8sllm_resolve_ids(int* out, const int* ids, const int* src, const int* prev, int n, hipStream_t s);
-int k8sllm_rope_cache(void* qkv, long qkv_stride, const int* positions, const float* cos_sin, void* k_cache,
+int k8sllm_rope_cache(void* qkv, long qkv_stride, const int* positions, const float* cos_sin, int max_pos, void* k_cache,
                       void* v_cache, const int* slot_mapping, long T, int Hq, int Hkv, int D, int block_size,
                       int apply_rope, const float* partial, int S, hipStream_t s);
 int k8sllm_paged_decode(void* out, long out_stride, float* part_out, float* part_ml, const void* q, long q_stride,
@@ -173,6 +173,7 @@ void rope_and_cache(torch::Tensor qkv, torch::Tensor positions, torch::Tensor co
   TORCH_CHECK(qkv.stride(-1) == 1 && qkv.dim() == 2, "qkv must be [T, (Hq+2Hkv)*D] with unit inner stride");
   TORCH_CHECK(qkv.size(1) >= (Hq + 2 * Hkv) * D, "qkv width");
   TORCH_CHECK(cos_sin.scalar_type() == torch::kFloat32 && cos_sin.is_contiguous() && cos_sin.size(1) == D, "cos_sin");
+  TORCH_CHECK(!apply_rope || cos_sin.size(0) > 0, "cos_sin is empty");
   const bool has_cache = slot_mapping.numel() > 0;
   int block_size = 16;
   if (has_cache) {
@@ -190,7 +191,7 @@ void rope_and_cache(torch::Tensor qkv, torch::Tensor positions, torch::Tensor co
     pp = partial->data_ptr<float>();
   }
   check(k8sllm_rope_cache(qkv.data_ptr(), qkv.stride(0), positions.data_ptr<int>(), cos_sin.data_ptr<float>(),
-                          has_cache ? k_cache.data_ptr() : nullptr, has_cache ? v_cache.data_ptr() : nullptr,
+                          (int)cos_sin.size(0), has_cache ? k_cache.data_ptr() : nullptr, has_cache ? v_cache.data_ptr() : nullptr,
                           has_cache ? slot_mapping.data_ptr<int>() : nullptr, qkv.size(0), (int)Hq, (int)Hkv, (int)D,
                           block_size, apply_rope ? 1 : 0, pp, (int)S, cur()),
         "rope_and_cache");

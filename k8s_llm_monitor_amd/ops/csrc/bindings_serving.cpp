@@ -8,6 +8,10 @@
 #include <cmath>
 
 extern "C" {
+int k8sllm_reduce_slabs(void* out, const float* partial, int S, long n, hipStream_t s);
+int k8sllm_rope_cache(void* qkv, long qkv_stride, const int* positions, const float* cos_sin, int max_pos, void* k_cache, void* v_cache,
+                      const int* slot_mapping, long T, int Hq, int Hkv, int D, int block_size, int apply_rope, const float* partial, int S,
+                      hipStream_t s);
 int k8sllm_kv8_write(const void* qkv, long stride, const int* slots, void* k, void* v, float* scales, int T, int Hq, int Hkv, int D, int pages,
                      hipStream_t s);
 int k8sllm_kv8_decode(void* out, long out_stride, float* part_o, float* part_ml, const void* q, long q_stride, void* k, void* v, float* scales,
@@ -108,7 +112,9 @@ struct Table {
 
 void positive(const Call& c, double scale) { TORCH_CHECK(scale > 0 && std::isfinite(scale), c.what, ": scale must be positive, is ", scale); }
 
-void kv8_write(Tensor qkv, Tensor slots, Tensor k, Tensor v, Tensor scales, int64_t Hq, int64_t Hkv, int64_t D) {
+// Slab sum, rotation, write - nothing of it before every argument has been looked at
+void kv8_write(Tensor qkv, c10::optional<Tensor> positions, c10::optional<Tensor> cos_sin, Tensor slots, Tensor k, Tensor v, Tensor scales,
+               int64_t Hq, int64_t Hkv, int64_t D, bool apply_rope, c10::optional<Tensor> partial, int64_t nslabs) {
   Call c(qkv, "rope_and_cache_kv8");
   const Heads h(c, Hq, Hkv, D);
   c.rows(qkv, (Hq + 2 * Hkv) * D, "qkv");
@@ -117,6 +123,24 @@ void kv8_write(Tensor qkv, Tensor slots, Tensor k, Tensor v, Tensor scales, int6
   const int64_t T = qkv.size(0);
   TORCH_CHECK(slots.numel() >= T && T < (1LL << 30), c.what, ": a slot for each row");
   TORCH_CHECK(T * Hkv < (1LL << 31), c.what, ": rows times kv heads below 2^31");  // waves are numbered in 32 bits
+  if (partial.has_value()) {
+    c.whole(*partial, torch::kFloat32, "partial");
+    TORCH_CHECK(qkv.size(1) == (Hq + 2 * Hkv) * D && qkv.is_contiguous() && nslabs >= 1 && nslabs < (1 << 20) &&
+                    partial->numel() >= nslabs * qkv.numel() && (uintptr_t)partial->data_ptr() % 16 == 0, c.what,
+                ": partial must hold nslabs x [T, (Hq + 2 Hkv) * D] from 16 bytes on, qkv be contiguous rows of that many columns");
+  }
+  if (apply_rope) {
+    TORCH_CHECK(positions.has_value() && cos_sin.has_value(), c.what, ": positions and cos_sin are needed");
+    c.whole(*positions, torch::kInt32, "positions");
+    c.whole(*cos_sin, torch::kFloat32, "cos_sin");
+    TORCH_CHECK(positions->numel() >= T && cos_sin->dim() == 2 && cos_sin->size(0) >= 1 && cos_sin->size(0) < (1LL << 31) && cos_sin->size(1) == D &&
+                    (uintptr_t)cos_sin->data_ptr() % 16 == 0, c.what, ": positions [T] and cos_sin [positions, D], from 16 bytes on");
+    TORCH_CHECK(T <= 1 || qkv.stride(0) >= (Hq + Hkv) * D, c.what, ": rows that are rotated in place must not overlap");
+  }
+  if (partial.has_value()) c.done(k8sllm_reduce_slabs(qkv.data_ptr(), partial->data_ptr<float>(), (int)nslabs, qkv.numel(), c.stream()));
+  if (apply_rope)
+    c.done(k8sllm_rope_cache(qkv.data_ptr(), qkv.stride(0), positions->data_ptr<int>(), cos_sin->data_ptr<float>(), (int)cos_sin->size(0), nullptr,
+                             nullptr, nullptr, T, h.Hq, h.Hkv, h.D, 16, 1, nullptr, 0, c.stream()));
   c.done(k8sllm_kv8_write(qkv.data_ptr(), qkv.stride(0), slots.data_ptr<int>(), cache.k, cache.v, cache.scales, (int)T, h.Hq, h.Hkv, h.D,
                           cache.pages, c.stream()));
 }

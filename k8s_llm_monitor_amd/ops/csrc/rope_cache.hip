@@ -35,7 +35,7 @@ __device__ __forceinline__ void slab_sum(const float* __restrict__ p, long slab_
 template <int D, bool SLAB>
 __global__ __launch_bounds__(128) void rope_cache_kernel(bf16_t* __restrict__ qkv, long qkv_stride,
                                                          const int* __restrict__ positions,
-                                                         const float* __restrict__ cos_sin,  // [max_pos][D]: cos | sin
+                                                         const float* __restrict__ cos_sin, int last_pos,  // [last_pos + 1][D]: cos | sin
                                                          bf16_t* __restrict__ k_cache, bf16_t* __restrict__ v_cache,
                                                          const int* __restrict__ slot_mapping, int Hq, int Hkv,
                                                          int block_size, int apply_rope, const float* __restrict__ partial,
@@ -76,7 +76,7 @@ __global__ __launch_bounds__(128) void rope_cache_kernel(bf16_t* __restrict__ qk
       }
     }
     if (apply_rope) {
-      const float* cs = cos_sin + (long)positions[t] * D;
+      const float* cs = cos_sin + (long)min(max(positions[t], 0), last_pos) * D;
       const float4 c = *reinterpret_cast<const float4*>(cs + p);
       const float4 s = *reinterpret_cast<const float4*>(cs + HALF + p);
       const float cc[4] = {c.x, c.y, c.z, c.w}, ss[4] = {s.x, s.y, s.z, s.w};
@@ -204,8 +204,8 @@ __global__ __launch_bounds__(256) void kv_cache_write_kernel(const bf16_t* __res
 
 using namespace k8sllm;
 
-extern "C" int k8sllm_rope_cache(void* qkv, long qkv_stride, const int* positions, const float* cos_sin, void* k_cache,
-                                 void* v_cache, const int* slot_mapping, long T, int Hq, int Hkv, int D,
+extern "C" int k8sllm_rope_cache(void* qkv, long qkv_stride, const int* positions, const float* cos_sin, int max_pos,
+                                 void* k_cache, void* v_cache, const int* slot_mapping, long T, int Hq, int Hkv, int D,
                                  int block_size, int apply_rope, const float* partial, int S, hipStream_t s) {
   if (T <= 0) return 0;
   if (D != 128 && D != 64) return -1;
@@ -219,7 +219,7 @@ extern "C" int k8sllm_rope_cache(void* qkv, long qkv_stride, const int* position
   const bool skip_rope = runs && !apply_rope;
 #define K8S_ROPE(DV, SL)                                                                                       \
   hipLaunchKernelGGL((rope_cache_kernel<DV, SL>), grid, dim3(128), 0, s, (bf16_t*)qkv, qkv_stride, positions,  \
-                     cos_sin, (bf16_t*)k_cache, (bf16_t*)v_cache, rope_slots, Hq, Hkv, block_size, apply_rope,   \
+                     cos_sin, max_pos - 1, (bf16_t*)k_cache, (bf16_t*)v_cache, rope_slots, Hq, Hkv, block_size, apply_rope,   \
                      partial, S, (int)T)
   if (skip_rope) {
   } else if (D == 128) {

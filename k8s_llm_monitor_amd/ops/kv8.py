@@ -17,7 +17,7 @@ from typing import NamedTuple, Optional
 
 import torch
 
-from . import MAX_SPLITS, _gpu, native, pack_activation, prefill_qblocks, reduce_slabs, rope_and_cache
+from . import MAX_SPLITS, _gpu, native, pack_activation, prefill_qblocks
 from . import reference as ref
 
 PAGE = 16
@@ -55,7 +55,7 @@ def kv8_block_bytes(Hkv: int, D: int) -> int:
 
 def rope_and_cache_kv8(qkv: torch.Tensor, positions: torch.Tensor, cos_sin: torch.Tensor, cache: KV8, slot_mapping: torch.Tensor, Hq: int,
                        Hkv: int, D: int, apply_rope: bool = True, partial: Optional[torch.Tensor] = None, nslabs: int = 0) -> None:
-    """In place: rotate q and k inside the fused QKV rows (``apply_rope``); write k, v into the pages of ``slot_mapping`` [T] (page * 16 + token;
+    """In place: rotate q and k inside the fused QKV rows (``apply_rope``; ``positions`` are held to the ends of ``cos_sin``); write k, v into the pages of ``slot_mapping`` [T] (page * 16 + token;
     < 0: not written).  Rows of one page follow one another, in the order of their slots, and go on where the page ends: what it holds at lower
     offsets are earlier tokens of the sequence, and its scale stays theirs or grows.  ``partial``: the rows are first the sum of ``nslabs`` fp32
     split-K slabs [nslabs, T, (Hq + 2 Hkv) * D]."""
@@ -63,14 +63,17 @@ def rope_and_cache_kv8(qkv: torch.Tensor, positions: torch.Tensor, cos_sin: torc
     if partial is not None:
         if qkv.shape[1] != (Hq + 2 * Hkv) * D or not qkv.is_contiguous() or not 1 <= nslabs or partial.numel() < nslabs * qkv.numel():
             raise ValueError("rope_and_cache_kv8: partial must hold nslabs x [T, (Hq + 2 Hkv) * D], qkv be contiguous rows of that many columns")
-        reduce_slabs(partial, nslabs, T, (Hq + 2 * Hkv) * D, qkv.dtype, out=qkv)
-    if apply_rope:
-        rope_and_cache(qkv, positions, cos_sin, None, None, None, Hq, Hkv, D, True)
     if _gpu(qkv):
-        native().kv8_write(qkv, slot_mapping, cache.k, cache.v, cache.scales, Hq, Hkv, D)
+        native().kv8_write(qkv, positions if apply_rope else None, cos_sin if apply_rope else None, slot_mapping, cache.k, cache.v, cache.scales,
+                           Hq, Hkv, D, apply_rope, partial, nslabs)
         return
+    runs = _runs(cache, slot_mapping, T)  # (refuses before anything has changed)
+    if partial is not None:
+        qkv.copy_(partial.reshape(-1)[: nslabs * qkv.numel()].view(nslabs, *qkv.shape).sum(0))
+    if apply_rope:
+        _rotate(qkv, positions, cos_sin, Hq, Hkv, D)
     x = qkv[:, : (Hq + 2 * Hkv) * D].reshape(T, Hq + 2 * Hkv, D)
-    _write(cache, slot_mapping, x[:, Hq:Hq + Hkv], x[:, Hq + Hkv:])
+    _write(cache, runs, x[:, Hq:Hq + Hkv], x[:, Hq + Hkv:])
 
 
 def paged_decode_kv8(q: torch.Tensor, cache: KV8, block_tables: torch.Tensor, seq_lens: torch.Tensor, Hq: int, Hkv: int, D: int, scale: float,
@@ -103,10 +106,11 @@ def paged_decode_fused_kv8(slabs: torch.Tensor, nslabs: int, positions: torch.Te
         qkv = slabs.reshape(-1)[: nslabs * B * n].view(nslabs, B, n).sum(0).to(dtype)
         if slot_mapping is None:
             slot_mapping = torch.full((B,), -1, dtype=torch.int32)
-        ref.rope_and_cache(qkv, positions, cos_sin, None, None, None, Hq, Hkv, D, True)
+        runs = _runs(cache, slot_mapping, B)
+        _rotate(qkv, positions, cos_sin, Hq, Hkv, D)
         x = qkv.view(B, Hq + 2 * Hkv, D)
         kn, vn = x[:, Hq:Hq + Hkv], x[:, Hq + Hkv:]
-        _write(cache, slot_mapping, kn, vn)
+        _write(cache, runs, kn, vn)
         fresh = [i for i in range(B) if int(slot_mapping[i]) < 0 and int(seq_lens[i]) > 0]
         new = {i: (_as_written(kn[i]), _as_written(vn[i])) for i in fresh}  # not written, attended as if alone in its page
         return _out(_decode_cpu(qkv, cache, block_tables, seq_lens, Hq, Hkv, D, scale, new), out)
@@ -192,9 +196,16 @@ def _as_written(x: torch.Tensor) -> torch.Tensor:
     return codes_of(x, s).float() * s
 
 
-def _write(cache: KV8, slots: torch.Tensor, k_new: torch.Tensor, v_new: torch.Tensor) -> None:
-    n, hkv = cache.scales.shape[:2]
-    sm = slots[: k_new.shape[0]].long()
+def _rotate(qkv: torch.Tensor, positions: torch.Tensor, cos_sin: torch.Tensor, Hq: int, Hkv: int, D: int) -> None:
+    ref.rope_and_cache(qkv, positions[: qkv.shape[0]].clamp(0, cos_sin.shape[0] - 1), cos_sin, None, None, None, Hq, Hkv, D, True)
+
+
+def _runs(cache: KV8, slots: torch.Tensor, T: int) -> tuple:
+    """Of ``T`` rows: those that are written, their pages, each one's page among them and place in it, the first place of every page."""
+    n = cache.scales.shape[0]
+    if slots.numel() < T:
+        raise ValueError("rope_and_cache_kv8: a slot for each row")
+    sm = slots[:T].long()
     rows = ((sm >= 0) & (sm < n * PAGE)).nonzero()[:, 0]
     sm = sm[rows]
     pages, row = torch.unique(sm // PAGE, return_inverse=True)
@@ -203,6 +214,12 @@ def _write(cache: KV8, slots: torch.Tensor, k_new: torch.Tensor, v_new: torch.Te
     start = torch.full_like(pages, 1 << 62).scatter_reduce(0, row, rows, "amin")
     if not torch.equal(off - first[row], rows - start[row]):
         raise ValueError("rope_and_cache_kv8: rows of one page must follow one another in the order of their slots")
+    return rows, pages, row, off, first
+
+
+def _write(cache: KV8, runs: tuple, k_new: torch.Tensor, v_new: torch.Tensor) -> None:
+    hkv = cache.scales.shape[1]
+    rows, pages, row, off, first = runs
     earlier = torch.arange(PAGE) < first[:, None]  # [pages, 16]
     for j, (codes, x) in enumerate(((cache.k, k_new[rows].float()), (cache.v, v_new[rows].float()))):
         amax = torch.zeros(pages.numel(), hkv).scatter_reduce(0, row[:, None].expand(-1, hkv), _finite_max(x), "amax")

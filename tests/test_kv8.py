@@ -278,6 +278,43 @@ def test_write_refuses_rows_out_of_order_on_the_cpu():
                                    apply_rope=False)
 
 
+@pytest.mark.parametrize("dev", DEVICES)
+def test_write_of_positions_outside_the_table(dev):
+    """Positions are held to the rotation table's ends, in the write and in the fused step."""
+    hq, hkv, d, n = 2, 1, 128, 20
+    gen = torch.Generator().manual_seed(13)
+    raw = (torch.randn(4, hq + 2 * hkv, d, generator=gen)).bfloat16()
+    slots, cs = torch.tensor([0, 1, 16, 32], dtype=torch.int32, device=dev), table_of(d, dev, n)
+    out = []
+    for pos in ([-5, 19, 1 << 30, -(1 << 31)], [0, 19, 19, 0]):
+        cache, qkv = ops.kv8_cache(4, hkv, d, device=dev), raw.clone().view(4, -1).to(dev)
+        ops.rope_and_cache_kv8(qkv, torch.tensor(pos, dtype=torch.int32, device=dev), cs, cache, slots, hq, hkv, d)
+        step = ops.kv8_cache(4, hkv, d, device=dev)
+        o = ops.paged_decode_fused_kv8(raw.float().view(1, 4, -1).to(dev), 1, torch.tensor(pos, dtype=torch.int32, device=dev), cs,
+                                       torch.tensor([0, 16, 32, 48], dtype=torch.int32, device=dev), step,
+                                       torch.arange(4, dtype=torch.int32, device=dev)[:, None], torch.ones(4, dtype=torch.int32, device=dev), hq, hkv, d, 0.1)
+        out.append([qkv, cache.k.view(torch.uint8), cache.v.view(torch.uint8), o, step.k.view(torch.uint8)])
+    assert all(torch.equal(a, b) for a, b in zip(*out))
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+def test_a_refused_write_changes_nothing(dev):
+    """Arguments are looked at before the rows are summed and rotated."""
+    hq, hkv, d = 2, 1, 128
+    rows = torch.randn(3, (hq + 2 * hkv) * d, generator=torch.Generator().manual_seed(14)).bfloat16().to(dev)
+    pos, cs = torch.tensor([5, 6, 7], dtype=torch.int32, device=dev), table_of(d, dev)
+    i32 = lambda *v: torch.tensor(v, dtype=torch.int32, device=dev)  # noqa: E731
+    bad = [dict(slots=i32(0, 1))] + ([dict(slots=i32(1, 0, 2))] if dev == "cpu" else
+                                     [dict(cache=ops.kv8_cache(2, 3, d, device=dev)), dict(pos=pos[:2]), dict(cs=cs[:, :64]), dict(slots=i32(0, 1, 2).long())])
+    for k in bad:
+        for partial in (None, torch.ones(2, *rows.shape, device=dev)):
+            k = {**dict(slots=i32(0, 1, 2), cache=ops.kv8_cache(2, hkv, d, device=dev), pos=pos, cs=cs), **k}
+            qkv = rows.clone()
+            with pytest.raises((RuntimeError, ValueError)):
+                ops.rope_and_cache_kv8(qkv, k["pos"], k["cs"], k["cache"], k["slots"], hq, hkv, d, partial=partial, nslabs=2)
+            assert torch.equal(qkv, rows)
+
+
 # ---------------------------------------------------------------- single tokens
 
 SHAPES = [(1, 1, 128), (8, 8, 64), (32, 8, 128), (7, 1, 128), (28, 4, 128), (16, 1, 64), (10, 2, 64)]
