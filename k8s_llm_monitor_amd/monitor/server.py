@@ -595,20 +595,22 @@ def _only(method: str, allowed: str) -> None:
 def _chat_controls(d: dict) -> dict:
     """SamplingParams' fields from a chat request's presence_penalty, frequency_penalty, repetition_penalty and logit_bias (token ids as JSON
     keys); 400 for values of another type."""
-    c = {}
-    for k in ("presence_penalty", "frequency_penalty", "repetition_penalty"):
-        if d.get(k) is not None:
-            if not isinstance(d[k], (int, float)) or isinstance(d[k], bool):
-                raise http_error(400, f"{k} must be a number")
-            try:
-                c[k] = float(d[k])
-            except OverflowError:  # a whole number of hundreds of digits
-                raise http_error(400, f"{k} is too large") from None
-    if d.get("logit_bias"):
+    def number(k, x):
+        if not isinstance(x, (int, float)) or isinstance(x, bool):
+            raise http_error(400, f"{k} must be a number")
         try:
-            c["logit_bias"] = {int(t): float(x) for t, x in d["logit_bias"].items()}
-        except (AttributeError, TypeError, ValueError, OverflowError):
-            raise http_error(400, "logit_bias must map token ids to numbers") from None
+            return float(x)
+        except OverflowError:  # a whole number of hundreds of digits
+            raise http_error(400, f"{k} is too large") from None
+
+    c = {k: number(k, d[k]) for k in ("presence_penalty", "frequency_penalty", "repetition_penalty") if d.get(k) is not None}
+    bias = d.get("logit_bias")
+    if bias is not None:
+        # (ids of at most 9 digits, written one way: none twice)
+        if not isinstance(bias, dict) or not all(len(t) < 10 and t.isascii() and t.isdigit() and str(int(t)) == t for t in bias):
+            raise http_error(400, "logit_bias must map token ids to numbers")
+        if bias:
+            c["logit_bias"] = {int(t): number("logit_bias", x) for t, x in bias.items()}
     return c
 
 

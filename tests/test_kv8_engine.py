@@ -320,3 +320,12 @@ def test_requests_that_allow_no_token_are_refused():
         few.add_request([5, 6], SamplingParams(logit_bias=dict.fromkeys(range(few.model_cfg.vocab_size), out)))
     s = e.add_request([5, 6], SamplingParams(max_tokens=3, temperature=0.9, ignore_eos=True, allowed_token_ids=(5, 6), logit_bias={5: out}))
     assert drain(e, [s])[0] == [6] * 3
+
+
+@pytest.mark.parametrize("bias", [[], 0, False, "", "7", {"7": "5"}, {"7": "inf"}, {"7": True}, {"7": None}, {"07": 1}, {" 7": 1}, {"1_0": 1}, {"-1": 1}, {"7.0": 1}])
+def test_chat_biases_of_another_type_are_bad_requests(bias):
+    from k8s_llm_monitor_amd.monitor.server import _chat_controls
+    with pytest.raises(Exception) as err:
+        _chat_controls({"logit_bias": bias})
+    assert err.value.code == 400
+    assert _chat_controls({"logit_bias": {}}) == _chat_controls({"logit_bias": None}) == {}
