@@ -32,7 +32,7 @@ class LogitControls(NamedTuple):
     def set(self, slot: int, prompt_len: int, repetition: float = 1.0, presence: float = 0.0, frequency: float = 0.0,
             bias: Optional[dict] = None, allowed: Optional[Iterable[int]] = None) -> None:
         """Fills a slot: the penalties, ``bias`` {token: addend}, ``allowed`` token ids (None: all).  A few small copies to the device, in the
-        order of the current stream."""
+        order of the current stream; the host does not wait for what runs there."""
         if not 0 <= slot < self.params.shape[0]:
             raise ValueError(f"LogitControls.set: slot {slot} of {self.params.shape[0]}")
         check_controls(repetition, presence, frequency, bias)
@@ -40,17 +40,24 @@ class LogitControls(NamedTuple):
         bias = bias or {}
         if len(bias) > m:
             raise ValueError(f"LogitControls.set: {len(bias)} biased tokens, room for {m}")
-        if allowed is not None:
-            self.masks[slot] = allowed_mask(allowed, words * 32).to(self.masks.device)
+        n = len(bias)
+        mask = allowed_mask(allowed, words * 32) if allowed is not None else None
+        # pinned memory, the allocator's own until the copies out of it are done: a copy from pageable memory would wait for the stream
+        stage = torch.empty(5 + 2 * m + (words if mask is not None else 0), dtype=torch.int32, pin_memory=self.params.is_cuda)
+        info, params, ids, vals = stage[:2], stage[2:5].view(torch.float32), stage[5:5 + m], stage[5 + m:5 + 2 * m].view(torch.float32)
+        info.copy_(torch.tensor([prompt_len, int(mask is not None)], dtype=torch.int32))
+        params.copy_(torch.tensor([repetition, presence, frequency], dtype=torch.float32))
+        ids[:n] = torch.tensor([int(t) for t in bias], dtype=torch.int32)
+        ids[n:] = -1
+        vals[:n] = torch.tensor([float(x) for x in bias.values()], dtype=torch.float32)
+        vals[n:] = 0
+        if mask is not None:
+            self.masks[slot].copy_(stage[5 + 2 * m:].copy_(mask), non_blocking=True)
         if m:
-            ids = torch.full((m,), -1, dtype=torch.int32)
-            vals = torch.zeros(m)
-            for j, (t, x) in enumerate(bias.items()):
-                ids[j], vals[j] = int(t), float(x)
-            self.bias_ids[slot] = ids.to(self.bias_ids.device)
-            self.bias_vals[slot] = vals.to(self.bias_vals.device)
-        self.params[slot] = torch.tensor([repetition, presence, frequency], dtype=torch.float32).to(self.params.device)
-        self.info[slot] = torch.tensor([prompt_len, int(allowed is not None)], dtype=torch.int32).to(self.info.device)
+            self.bias_ids[slot].copy_(ids, non_blocking=True)
+            self.bias_vals[slot].copy_(vals, non_blocking=True)
+        self.params[slot].copy_(params, non_blocking=True)
+        self.info[slot].copy_(info, non_blocking=True)
 
 
 def check_controls(repetition: float = 1.0, presence: float = 0.0, frequency: float = 0.0, bias: Optional[dict] = None) -> None:

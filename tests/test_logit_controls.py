@@ -284,3 +284,28 @@ def test_sampling_of_infinite_logits(dev, top_k, top_p, temp):
     for _ in range(10):
         t = ops.sample(x, full(temp, torch.float32), full(top_k, torch.int32), full(top_p, torch.float32), rng, advance=True).tolist()
         assert t[:3] == [77, 9, 0] and 500 <= t[3] < V
+
+
+@pytest.mark.gpu
+def test_filling_slots_does_not_wait_for_the_stream():
+    """Behind products that are still running, slots are filled without waiting for them; what is read after them is right, slot by slot."""
+    V = 5003
+    ctl = [(i, f32(1.1 + 0.1 * i), 0.5, 0.25 * i, {j: float(j - i) for j in range(i)}, range(i, V, 3) if i % 2 else None) for i in range(6)]
+    c = controls("cuda", V, ctl)
+    want = [t.clone() for t in c]
+    a = torch.randn(8192, 8192, device="cuda").bfloat16()
+    c = controls("cuda", V, ctl)  # (the library's product and the pinned blocks are there)
+    a @ a
+    torch.cuda.synchronize()
+    for _ in range(60):
+        b = a @ a
+    end = torch.cuda.Event()
+    end.record()
+    fresh = [torch.empty_like(t).copy_(t) for t in ops.logit_controls(len(ctl), V, 8, device="cuda")]
+    c = ops.LogitControls(*fresh)
+    for i, (prompt, rep, pres, freq, bias, allowed) in enumerate(ctl):
+        c.set(i, prompt, rep, pres, freq, bias, allowed)
+    waited = end.query()
+    torch.cuda.synchronize()
+    assert not waited
+    assert all(torch.equal(x, y) for x, y in zip(c, want))
