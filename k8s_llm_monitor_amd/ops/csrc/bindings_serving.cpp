@@ -254,6 +254,19 @@ void kv8_prefill(Tensor out, Tensor qkv, Tensor cu, Tensor ctx, Tensor qb_seq, T
                             S > 1 ? pml.data_ptr<float>() : nullptr, c.stream()));
 }
 
+// Whether rows of `out` share memory with rows of `in` other than as one and the same view
+bool half_shared(const Tensor& out, const Tensor& in) {
+  const int64_t B = in.size(0), os = out.stride(0) * out.element_size(), is = in.stride(0) * in.element_size();
+  const int64_t ow = out.size(1) * out.element_size(), iw = in.size(1) * in.element_size(), d = (char*)out.data_ptr() - (char*)in.data_ptr();
+  if (d >= (B - 1) * is + iw || -d >= (B - 1) * os + ow) return false;
+  if (B > 1 && os != is) return true;
+  if (d == 0 && out.scalar_type() == in.scalar_type()) return false;
+  // row i of out begins d + (i - j) * is behind row j of in
+  for (int64_t k = -(B - 1); k < B; ++k)
+    if (d + k * is < iw && -(d + k * is) < ow) return true;
+  return false;
+}
+
 void logit_controls(Tensor out, Tensor logits, Tensor params, Tensor info, Tensor bias_ids, Tensor bias_vals, Tensor masks, Tensor rows, Tensor tokens,
                     Tensor table, Tensor lens) {
   Call c(logits, "control_logits");
@@ -267,6 +280,7 @@ void logit_controls(Tensor out, Tensor logits, Tensor params, Tensor info, Tenso
   TORCH_CHECK(B <= 1 || out.stride(0) >= V, c.what, ": rows of out must not overlap");
   TORCH_CHECK(B <= 65535, c.what, ": at most 65535 rows");
   if (B == 0 || V == 0) return;
+  TORCH_CHECK(!half_shared(out, logits), c.what, ": out shares memory with the logits and is not the same rows");
   c.whole(params, torch::kFloat32, "controls.params");
   c.whole(info, torch::kInt32, "controls.info");
   c.whole(bias_ids, torch::kInt32, "controls.bias_ids");

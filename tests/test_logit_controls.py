@@ -309,3 +309,35 @@ def test_filling_slots_does_not_wait_for_the_stream():
     torch.cuda.synchronize()
     assert not waited
     assert all(torch.equal(x, y) for x, y in zip(c, want))
+
+
+@pytest.mark.gpu
+def test_outputs_that_share_memory_with_the_logits():
+    """In place, or side by side in one buffer: right.  Anything between - shifted, of another type, rows of another distance - is refused."""
+    B, V, dev = 3, 5003, "cuda"
+    gen = torch.Generator().manual_seed(8)
+    ctl = [(2, f32(1.3), 0.5, 0.25, {7: 1.0}, range(0, V, 3))]
+    c, rows = controls(dev, V, ctl), torch.zeros(B, dtype=torch.int32, device=dev)
+    tokens = torch.randint(0, V, (4, 16), generator=gen).int()
+    table, lens = torch.tensor([[0, 1], [2, 3], [1, 2]], dtype=torch.int32), [20, 3, 32]
+    x = torch.randn(B, V, generator=gen)
+    want = plain(x, ctl, [0] * B, tokens, table.tolist(), lens)
+    args = (c, rows, tokens.to(dev), table.to(dev), torch.tensor(lens, dtype=torch.int32, device=dev))
+    wide = torch.zeros(B, 2 * V + 5, device=dev)
+    left, right = wide[:, :V], wide[:, V + 5:]
+    for src, out in ((left, right), (right, left), (left, left)):
+        src.copy_(x)
+        ops.control_logits(src, *args, out=out)
+        check(out, *want)
+    flat = torch.zeros(2 * B * V + 16, device=dev)
+    a = flat[: B * V].view(B, V)
+    for out in (flat[4:4 + B * V].view(B, V), flat[V:V + B * V].view(B, V), flat.as_strided((B, V), (2 * V, 1)), flat.as_strided((B, V), (V, 1), 2 * V)):
+        with pytest.raises(RuntimeError, match="memory"):
+            ops.control_logits(a, *args, out=out)
+    with pytest.raises(RuntimeError, match="memory"):
+        ops.control_logits(flat[: B * V].view(torch.bfloat16)[: B * V].view(B, V), *args, out=a)
+    a.copy_(x)
+    out = flat[B * V:2 * B * V].view(B, V)  # from where the logits end
+    ops.control_logits(a, *args, out=out)
+    check(out, *want)
+    torch.cuda.synchronize()
