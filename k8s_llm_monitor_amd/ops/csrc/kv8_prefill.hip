@@ -72,12 +72,12 @@ __global__ __launch_bounds__(512, 2) void kv8_prefill_kernel(const Kv8Prefill a)
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int r32 = lane & 31, hh = lane >> 5;
   const int cst = __builtin_amdgcn_readfirstlane(max(0, min(a.ctx[seq], a.table_width * kPage - L)));  // keys never pass the table
-  const int LK = cst + L, last_page = min((LK - 1) >> 4, a.table_width - 1);
+  const int LK = min(cst + L, a.table_width * kPage), last_page = (LK - 1) >> 4;  // (a chunk longer than the table: its last rows see all of it)
   const int f = f0 + 32 * wave + r32;
   const bool mine = f < pairs;
   const int row = qs + (mine ? f / G : 0), hq = kvh * G + (mine ? f % G : 0);
   // (divisions are done in vector registers: what branches hang on goes back to scalar ones)
-  const int wave_first = __builtin_amdgcn_readfirstlane(cst + qs + (f0 + 32 * wave) / G);  // position of the wave's first row
+  const int wave_first = __builtin_amdgcn_readfirstlane(min(cst + qs + (f0 + 32 * wave) / G, LK - 1));  // the last key that the wave's first row sees
   const bool busy = f0 + 32 * wave < pairs;
   const int wave_last = cst + qs + (min(pairs, f0 + 32 * wave + 32) - 1) / G;
   const int tiles = (cst + qs + (min(pairs, f0 + 256) - 1) / G) / kTile + 1;
@@ -251,7 +251,7 @@ __global__ __launch_bounds__(512, 2) void kv8_prefill_kernel(const Kv8Prefill a)
     }
     __builtin_amdgcn_sched_barrier(0);
     if (t * kTile + kTile - 1 > wave_first) {  // keys past this lane's row (uniform branch)
-      const int lim = cst + row - t * kTile - 4 * hh;
+      const int lim = min(cst + row, LK - 1) - t * kTile - 4 * hh;
 #pragma unroll
       for (int i = 0; i < 2; ++i)
 #pragma unroll

@@ -9,7 +9,7 @@ nothing but codes that become subnormal.  Numbers that are not finite become NaN
 The operators stand beside ``rope_and_cache``, ``paged_decode``, ``paged_decode_fused`` and ``flash_prefill``, with the cache as one argument.
 Head sizes 64 and 128 (the fused form: 128), any 1 to 16 query heads a kv head.  GPU: bf16 rows, the kernels of ``csrc/kv8_*.hip``; CPU: any
 floating rows, the forms below.  What a page holds behind a sequence's end does not matter, NaN included; page numbers outside the cache are
-held to its ends, block tables end a sequence, slots outside the cache are not written.
+held to its ends, block tables end a sequence (rows of a chunk that is longer than its table see all that it holds), slots outside the cache are not written.
 """
 from __future__ import annotations
 
@@ -271,7 +271,10 @@ def _prefill_cpu(qkv, cu_seqlens, ctx_start, cache, block_tables, Hq, Hkv, D, sc
     for i in range(len(cu) - 1):
         a, b = cu[i], cu[i + 1]
         if b > a:
-            c = max(0, min(cs[i], block_tables.shape[1] * PAGE - (b - a)))
-            k, v = gather_kv8(cache, block_tables[i], c + b - a)
-            out[a:b] = ref.attention(qkv[a:b, : Hq * D].view(b - a, Hq, D), k, v, scale, causal=True).reshape(b - a, -1).to(qkv.dtype)
+            n = min(b - a, block_tables.shape[1] * PAGE)
+            c = max(0, min(cs[i], block_tables.shape[1] * PAGE - n))
+            k, v = gather_kv8(cache, block_tables[i], c + n)
+            for r0, r1, causal in ((a, a + n, True), (a + n, b, False)):
+                q = qkv[r0:r1, : Hq * D].reshape(r1 - r0, Hq, D)
+                out[r0:r1] = ref.attention(q, k, v, scale, causal=causal).reshape(r1 - r0, Hq * D).to(qkv.dtype)
     return out

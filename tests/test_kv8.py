@@ -498,6 +498,25 @@ def test_prefill(dev, hq, hkv, d):
 
 
 @pytest.mark.parametrize("dev", DEVICES)
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("width,ctx,new", [(1, 0, 40), (3, 0, 49), (2, 9, 300), (5, 70, 30), (20, 300, 40)])
+def test_prefill_of_chunks_longer_than_their_table(dev, d, width, ctx, new):
+    """The table ends the sequence: a context that does not fit is cut, rows behind the end see all that the table holds, and nothing twice."""
+    hq, hkv = 4, 2
+    gen = torch.Generator().manual_seed(width + new)
+    n = 16 * width
+    cache, table, book = filled(gen, dev, [n], hkv, d)
+    q = rand(gen, new, hq, d).bfloat16()
+    i32 = lambda *v: torch.tensor(v, dtype=torch.int32, device=dev)  # noqa: E731
+    got = ops.flash_prefill_kv8(q.view(new, -1).to(dev), i32(0, new), i32(ctx), cache, table.to(dev), hq, hkv, d, 0.1)
+    fit = min(new, n)
+    k, v = book.tokens(table[0], n)
+    first = max(0, min(ctx, n - fit))
+    want = [attend(q[:fit].double(), k, v, 0.1, first)] + [attend(q[i:i + 1].double(), k, v, 0.1, n - 1) for i in range(fit, new)]
+    check_attention(got, *(torch.cat(w) for w in zip(*want)))
+
+
+@pytest.mark.parametrize("dev", DEVICES)
 def test_prefill_few_rows_behind_a_long_context(dev):
     """One split of keys each: 3 and 40 rows behind contexts of 2000 and 9 tokens."""
     hq, hkv, d = 8, 2, 128
