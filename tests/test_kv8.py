@@ -269,6 +269,34 @@ def test_write_many_rows_rotated_and_from_slabs(dev, T):
     book.check(cache)
 
 
+@pytest.mark.parametrize("dev", DEVICES)
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("T", [513, 2049, 4097, 5003])
+def test_write_of_large_steps(dev, d, T):
+    """Row counts on both sides of where a wave takes 2, 8 and 16 of them: sequences of 1 to 60 rows that begin anywhere in a page, so that
+    runs lie across every border of 8 and 16 rows, rows without a slot between some of them, the last sequence cut by the end."""
+    hkv = 2
+    gen = torch.Generator().manual_seed(T + d)
+    at = lambda n: int(torch.randint(0, n, (1,), generator=gen))  # noqa: E731
+    slots, page = [], 0
+    while len(slots) < T:
+        n, first = 1 + at(60), at(16)
+        slots += range(page * 16 + first, page * 16 + first + n)
+        page += (first + n + 15) // 16
+        slots += [-1] * (at(4) if at(3) == 0 else 0)
+    order = torch.randperm(page, generator=gen)
+    slots = torch.tensor([-1 if s < 0 else int(order[s // 16]) * 16 + s % 16 for s in slots[:T]], dtype=torch.int32)
+    cache = ops.kv8_cache(page, hkv, d, device=dev)
+    garbage(cache, gen)
+    book = Book(cache)
+    x = rand(gen, T, 3 * hkv, d, spread=1.0).bfloat16()
+    wide = torch.zeros(T, 3 * hkv * d + 8, dtype=torch.bfloat16)
+    wide[:, : 3 * hkv * d] = x.view(T, -1)
+    ops.rope_and_cache_kv8(wide.to(dev), None, None, cache, slots.to(dev), hkv, hkv, d, apply_rope=False)
+    book.write(slots, x[:, hkv:2 * hkv].double(), x[:, 2 * hkv:].double())
+    book.check(cache)
+
+
 def test_write_refuses_rows_out_of_order_on_the_cpu():
     cache = ops.kv8_cache(4, 1, 64)
     qkv = torch.zeros(3, 192, dtype=torch.bfloat16)
@@ -550,6 +578,44 @@ def test_prefill_nan_counts_for_rows_that_see_it(ctx, new):
     cu = torch.tensor([0, new], dtype=torch.int32)
     got = ops.flash_prefill_kv8(q.view(new, -1).cuda(), cu.cuda(), torch.tensor([ctx], dtype=torch.int32).cuda(), cache, table.cuda(), hq, hkv, d, 0.1)
     want, size = attend(q.double(), *book2.tokens(table[0], n), 0.1, ctx)
+    _, size = attend(q.double(), *book.tokens(table[0], n), 0.1, ctx)
+    assert bool(want.isnan().any()) and not bool(want[: new // 3].isnan().any())
+    check_attention(got, want, size)
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+@pytest.mark.parametrize("hq,hkv,d", [(8, 8, 64), (16, 1, 64), (16, 1, 128), (7, 1, 128), (32, 8, 128)])
+def test_prefill_with_split_keys_of_every_form(dev, hq, hkv, d):
+    """Both head sizes, one and several groups of 256 (row, head) pairs a q-block, a split that ends behind the rows' last key."""
+    gen = torch.Generator().manual_seed(hq + d)
+    ctx, new = [1800, 3, 1021], [44, 40, 17]
+    cache, table, book = filled(gen, dev, [a + b for a, b in zip(ctx, new)], hkv, d)
+    q = rand(gen, sum(new), hq, d).bfloat16()
+    cu = torch.tensor([0, *itertools.accumulate(new)], dtype=torch.int32)
+    got = ops.flash_prefill_kv8(q.view(sum(new), -1).to(dev), cu.to(dev), torch.tensor(ctx, dtype=torch.int32, device=dev), cache, table.to(dev), hq,
+                                hkv, d, 0.1)
+    want = [attend(q[int(cu[i]):int(cu[i + 1])].double(), *book.tokens(table[i], a + b), 0.1, a) for i, (a, b) in enumerate(zip(ctx, new))]
+    check_attention(got, *(torch.cat(w) for w in zip(*want)))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("ctx,new", [(0, 200), (50, 100), (1500, 20)])
+def test_prefill_nan_counts_for_rows_that_see_it_at_head_size_64(ctx, new):
+    hq, hkv, d = 4, 2, 64
+    gen = torch.Generator().manual_seed(ctx + new + 1)
+    n = ctx + new
+    cache, table, book = filled(gen, "cuda", [n], hkv, d)
+    bad_v, bad_k = ctx + new // 3, ctx + new - 5
+    page, off = int(table[0, bad_v // 16]), bad_v % 16
+    cache.v.view(torch.uint8)[page, 0, 61, off] = NAN_CODE
+    cache.v.view(torch.uint8)[page, 1, 3, off] = 0xFF
+    page, off = int(table[0, bad_k // 16]), bad_k % 16
+    cache.k.view(torch.uint8)[page, 1, 2, off, 9] = NAN_CODE
+    book2 = Book(cache)
+    q = rand(gen, new, hq, d).bfloat16()
+    cu = torch.tensor([0, new], dtype=torch.int32)
+    got = ops.flash_prefill_kv8(q.view(new, -1).cuda(), cu.cuda(), torch.tensor([ctx], dtype=torch.int32).cuda(), cache, table.cuda(), hq, hkv, d, 0.1)
+    want, _ = attend(q.double(), *book2.tokens(table[0], n), 0.1, ctx)
     _, size = attend(q.double(), *book.tokens(table[0], n), 0.1, ctx)
     assert bool(want.isnan().any()) and not bool(want[: new // 3].isnan().any())
     check_attention(got, want, size)

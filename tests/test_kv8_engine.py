@@ -329,3 +329,116 @@ def test_chat_biases_of_another_type_are_bad_requests(bias):
         _chat_controls({"logit_bias": bias})
     assert err.value.code == 400
     assert _chat_controls({"logit_bias": {}}) == _chat_controls({"logit_bias": None}) == {}
+
+
+# ---------------------------------------------------------------- whole engines, by what they leave in their pages
+
+def held(e, s):
+    """What a sequence's pages stand for: [layers, 2, tokens, Hkv, D] of the tokens whose rows have run."""
+    from k8s_llm_monitor_amd.ops import KV8
+    from k8s_llm_monitor_amd.ops.kv8 import gather_kv8
+    table, n = torch.tensor(s.block_table), s.num_tokens - 1
+    rows = [gather_kv8(KV8(*(t.cpu() for t in e.runner.kv[i])), table, n) for i in range(len(e.runner.kv))]
+    return torch.stack([torch.stack(r) for r in rows])
+
+
+def run_forced(e, arrivals, steps=12):
+    """Requests that arrive every other step, each fed tokens of its own at every step: what their pages hold one token before the end."""
+    par = SamplingParams(max_tokens=steps, **GREEDY)
+    seqs, out = [], {}
+    while len(out) < len(arrivals):
+        if len(seqs) < len(arrivals):
+            seqs.append(e.add_request(arrivals[len(seqs)], par))
+        for _ in range(2):
+            e.step()
+            for i, s in enumerate(seqs):
+                if s.output_ids and not s.finish_reason:
+                    s.output_ids[-1] = 3 + (31 * i + 7 * len(s.output_ids)) % 240
+                    if len(s.output_ids) == steps - 1:
+                        out[i] = held(e, s)
+    return [out[i] for i in range(len(arrivals))]
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+def test_pages_of_chunks_mixed_steps_and_prefix_hits(dev):
+    """Together, with chunks, mixed steps and a cached prefix, sequences leave in their pages what each leaves alone, whole.  Rows of other steps go through
+    other matrix kernels: at most 12 roundings a layer of half a bf16 step (2^-9) in two layers, 0.047 of the norm, and where rows differ by that a code in
+    32 is the neighbouring one, 2^-3 off, 0.022 of the norm.  (fp32 rows: 2^-10 as above.)  A wrong page or position is off by the norm itself."""
+    kw = dict(kv_cache_dtype="fp8", pipeline=False)
+    arrivals = [prompt(100, 1), prompt(17, 2), prompt(100, 1)[:64] + prompt(30, 3), prompt(5, 4)]
+    e = engine(dev, max_prefill_tokens=48, mixed_prefill_tokens=32, **kw)
+    together = run_forced(e, arrivals)
+    assert e.runner.n_steps.get("mixed", 0) > 0 and e.runner.n_steps["prefill_context_tokens"] >= 64
+    for i, p in enumerate(arrivals):
+        alone = run_forced(engine(dev, prefix_caching=False, **kw), [arrivals[j] if j == i else [3] for j in range(len(arrivals))])[i]
+        assert alone.shape == together[i].shape
+        for a, b in zip(alone.flatten(0, 1), together[i].flatten(0, 1)):
+            assert float((a - b).norm() / a.norm()) <= (0.07 if dev == "cuda" else 2.0 ** -10)
+
+
+def _tp_worker(rank, world, port, q):
+    import os
+    os.environ.update(MASTER_ADDR="127.0.0.1", MASTER_PORT=str(port), RANK=str(rank), WORLD_SIZE=str(world), LOCAL_RANK=str(rank))
+    torch.set_num_threads(2)
+    from k8s_llm_monitor_amd.engine.runner import ModelRunner
+    from k8s_llm_monitor_amd.parallel.state import ParallelState, destroy, init_parallel
+    try:
+        ps = init_parallel(tp_size=world, device="cpu")
+        micro = []
+        # steps of several prompts in two micro-batches, however few their rows
+        ModelRunner._micro_split = staticmethod(lambda cu, nd, min_rows=0: micro.append(1) or 1 if len(cu) > 2 and not nd else 0)
+        cfg = EngineConfig(model="llama-tiny-d128", max_num_seqs=4, max_model_len=512, num_blocks=128, use_graphs=False, dtype="float32",
+                           kv_cache_dtype="fp8", keep_logits=True, max_prefill_tokens=200)
+        shared = prompt(64, 1)
+        asks = [[prompt(100, 5), prompt(17, 2), shared], [shared + prompt(30, 3), prompt(5, 4)], [prompt(300, 6)]]
+
+        def drive(e):
+            par, got = SamplingParams(max_tokens=3, **GREEDY), []
+            for ask in asks:
+                seqs = [e.add_request(p, par) for p in ask]
+                while not all(s.output_ids for s in seqs):
+                    e.step()
+                got.append(e.runner.last_logits.float().clone())
+                drain(e, seqs)
+            return got
+        e = LLMEngine(cfg, device="cpu", pstate=ps)
+        got = None
+        if ps.tp_rank == 0:
+            got = drive(e)
+            e.stop_workers()
+        else:
+            e.worker_loop()
+        e.bus.close()
+        n = len(micro)
+        if got is not None:
+            want = drive(LLMEngine(cfg, device="cpu", pstate=ParallelState()))
+            q.put((rank, [float((a - b).norm() / b.norm()) for a, b in zip(got, want)], n))
+        else:
+            q.put((rank, [0.0], n))
+        destroy()
+    except Exception as err:  # noqa: BLE001
+        import traceback
+        q.put((rank, repr(err) + traceback.format_exc(), 0))
+
+
+@pytest.mark.parametrize("world", [2, 4])
+def test_tensor_parallel_engines(world):
+    """Heads split over ranks (4 ranks: kv heads on two each), micro-batches, chunks, a prefix hit: the prompts' logits are those of one rank (the bound: as
+    above, the sums over ranks are rounded in another order)."""
+    import socket
+
+    import torch.multiprocessing as mp
+    with socket.socket() as s:
+        s.bind(("127.0.0.1", 0))
+        port = s.getsockname()[1]
+    ctx = mp.get_context("spawn")
+    q = ctx.Queue()
+    procs = [ctx.Process(target=_tp_worker, args=(r, world, port, q)) for r in range(world)]
+    for p in procs:
+        p.start()
+    res = [q.get(timeout=300) for _ in procs]
+    for p in procs:
+        p.join(60)
+    for rank, errs, micro in res:
+        assert not isinstance(errs, str), errs
+        assert max(errs) <= 2.0 ** -10 and micro > 0
