@@ -133,8 +133,12 @@ def flash_prefill_kv8(qkv: torch.Tensor, cu_seqlens: torch.Tensor, ctx_start: to
         r = _prefill_cpu(qkv, cu_seqlens, ctx_start, cache, block_tables, Hq, Hkv, D, scale)
         if out is None:
             return r
-        n = int(cu_seqlens[-1])
-        out[:n] = r[:n]
+        cu = cu_seqlens.tolist()
+        named = qblocks if qblocks is not None else prefill_qblocks(cu)
+        for i, at in zip(*(x.tolist() if torch.is_tensor(x) else x for x in named)):
+            if 0 <= i < len(cu) - 1 and at >= 0:
+                rows = slice(cu[i] + at, min(cu[i] + at + 128, cu[i + 1]))
+                out[rows] = r[rows]
         return out
     if qblocks is None:
         if ctx_start.numel() < cu_seqlens.numel() - 1:

@@ -584,6 +584,29 @@ def test_prefill_nan_counts_for_rows_that_see_it(ctx, new):
 
 
 @pytest.mark.parametrize("dev", DEVICES)
+def test_prefill_leaves_rows_that_no_block_names(dev):
+    """Of the rows ahead of the first sequence, of a sequence without a block and of one whose blocks are named in part, nothing is written."""
+    hq, hkv, d = 4, 2, 128
+    gen = torch.Generator().manual_seed(22)
+    new = [140, 20, 300]
+    cache, table, book = filled(gen, dev, new, hkv, d)
+    ahead = 3
+    q = rand(gen, ahead + sum(new), hq, d).bfloat16()
+    cu = torch.tensor([ahead + n for n in (0, *itertools.accumulate(new))], dtype=torch.int32)
+    i32 = lambda *v: torch.tensor(v, dtype=torch.int32, device=dev)  # noqa: E731
+    out = torch.full((len(q), hq * d), 7.0, dtype=torch.bfloat16, device=dev)
+    blocks = (i32(0, 2, 0, -1, 3), i32(0, 128, 128, 0, 0))  # (sequences that there are not: nothing)
+    ops.flash_prefill_kv8(q.view(len(q), -1).to(dev), cu.to(dev), i32(0, 0, 0), cache, table.to(dev), hq, hkv, d, 0.1, qblocks=blocks, out=out)
+    named = torch.zeros(len(q), dtype=torch.bool)
+    for i, first, n in ((0, 0, 140), (2, 128, 128)):
+        rows = slice(int(cu[i]) + first, int(cu[i]) + first + n)
+        named[rows] = True
+        want = attend(q[rows].double(), *(t[: first + n] for t in book.tokens(table[i], new[i])), 0.1, first)
+        check_attention(out[rows], *want)
+    assert bool((out[~named.to(dev)] == 7).all())
+
+
+@pytest.mark.parametrize("dev", DEVICES)
 @pytest.mark.parametrize("hq,hkv,d", [(8, 8, 64), (16, 1, 64), (16, 1, 128), (7, 1, 128), (32, 8, 128)])
 def test_prefill_with_split_keys_of_every_form(dev, hq, hkv, d):
     """Both head sizes, one and several groups of 256 (row, head) pairs a q-block, a split that ends behind the rows' last key."""
