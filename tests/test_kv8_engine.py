@@ -442,3 +442,25 @@ def test_tensor_parallel_engines(world):
     for rank, errs, micro in res:
         assert not isinstance(errs, str), errs
         assert max(errs) <= 2.0 ** -10 and micro > 0
+
+
+def _on_cpu(x):
+    if isinstance(x, torch.Tensor):
+        return x.cpu()
+    if isinstance(x, dict):
+        return {k: _on_cpu(v) for k, v in x.items()}
+    return type(x)(map(_on_cpu, x)) if isinstance(x, (list, tuple)) and type(x) in (list, tuple) else x
+
+
+@pytest.mark.gpu
+def test_gpt2_pages_on_the_gpu():
+    """GPT-2's heads (64 dims, no rotation, biases): with the same weights, the GPU's pages are the CPU's.  The bound: as above."""
+    kw = dict(model="gpt2-tiny", max_model_len=128, num_blocks=64, kv_cache_dtype="fp8", max_prefill_tokens=16, pipeline=False)
+    arrivals = [prompt(40, 3), prompt(7, 4), prompt(20, 5)]
+    e, c = engine("cuda", **kw), engine("cpu", dtype="bfloat16", **kw)
+    for name in ("embed", "pos_embed", "final_norm", "layers", "lm_head"):
+        if hasattr(e.model, name):
+            setattr(c.model, name, _on_cpu(getattr(e.model, name)))
+    for a, b in zip(run_forced(e, arrivals), run_forced(c, arrivals)):
+        for x, y in zip(a.flatten(0, 1), b.flatten(0, 1)):
+            assert float((x - y).norm() / y.norm()) <= 0.07
