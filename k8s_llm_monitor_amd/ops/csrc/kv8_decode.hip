@@ -20,10 +20,11 @@
 // FUSED (the decode step, D = 128): q, k and v of the new token are the sum of the qkv projection's split-K slabs, rounded to bf16, q and k
 // rotated.  The split that holds the sequence's end rounds k and v to the page's codes, attends to them from registers and, when all its
 // waves have read their pages, writes them; if the page's scale grows it rounds the earlier tokens' codes anew, for its own products too: the
-// answer is that of the write and the attention one after the other.
+// answer is that of the write and the attention one after the other.  (The rotation's products are rounded one by one here; rotations that fuse them into
+// the sums, as rope_and_cache's does, give the next bf16 number now and then.)
 //
 // Bound by memory: 64 x ~1.7 k tokens, 8 kv heads, 231 MB: 43 us, 5.3 TB/s (the same kernel without its products 41 to 43; a large sum reads 6.0);
-// 8 x 31 k tokens, 512 MB: 93 us; over the bf16 cache the first takes 79 us.  One sequence of 1.7 k tokens: 10 us, of one token 6.9,
+// 8 x 31 k tokens, 512 MB: 93 us; over the bf16 cache the first takes 79 us.  One sequence of 1.7 k tokens: 10 us, of one token 6.7,
 // a launch that does nothing 3 to 4.
 #include "kv8.h"
 

@@ -1,5 +1,6 @@
 // Causal attention of prompt chunks over the 8-bit pages (kv8.h): the queries are the new rows of the qkv buffer, all keys and values
-// - what came before and the chunk itself - are read from the pages, so that a prompt's answer does not depend on where it was cut.
+// - what came before and the chunk itself, whole prompts too - are read from the pages, so that a prompt's answer does not depend on where it was cut
+// (but for codes that become subnormal where a later chunk makes a page's scale grow) nor on what else is in the step.
 //
 // A workgroup takes one kv head and 256 (query row, head of the group) pairs, pair f = row * G + g, 32 to a wave: any group size fills
 // the 32-column MFMAs, and the heads of a row share every K / V tile.  Products are in the swapped orientation

@@ -148,7 +148,7 @@ __global__ __launch_bounds__(kLcThreads) void logit_controls_kernel(TO* out, lon
     __syncthreads();
   }
   const float* bv = c.bias_vals + (long)max(slot, 0) * c.n_bias;
-  const float inv = 1.f / rep;  // (a quotient for each token of a row's frequent ones is what the slowest workgroups would spend their time on)
+  const float inv = 1.f / rep;  // one rounding more, half a step of 32 bits (a quotient for each token of a row's frequent ones is what the slowest workgroups would spend their time on)
   auto one = [&](float f, uint32_t w) {
     const float count = (float)(w & kLcCount);
     if (w & (kLcPrompt | kLcCount)) f *= f > 0.f ? inv : rep;
